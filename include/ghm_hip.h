@@ -616,6 +616,77 @@ int ghm_tok_readout_bwd(const float* Z, const float* d_emb, const float* w_out, 
 int ghm_zsc_logits(const float* i_emb, int64_t n_rows, const float* t_emb, int D, const int32_t* proto_idx,
                    int n_class, int n_proto, const int32_t* n_list, int n_j, float* logits, void* stream);
 
+/* ---- token operators over a vocabulary of any size (csrc/ghm_token.hip) ---
+ * The large-vocabulary counterparts of ghm_ce_kl, ghm_tok_embed_fwd and ghm_wcolsum;
+ * the reference's vocabulary has 10 values and it has no counterpart of these.
+ *
+ * dtype: 0 f32, 1 bf16, 2 f16.  Logits rows r = 0 .. rows - 1 start at element
+ * (r / n_inner) * s_outer + (r % n_inner) * s_inner, V consecutive values each, at
+ * any element alignment.  id_bits / target_bits: 8 (unsigned), 32 or 64.  Statistics,
+ * sums and losses are f32; results do not depend on the launch's timing (no floating
+ * point atomics).  ws: scratch of at least the matching *_ws bytes (16-byte aligned,
+ * NULL where that is 0), not shared by calls that may run at the same time.
+ *
+ * A row whose target is ignore_index is padding: its logits are never read, its
+ * results and gradient are 0 (top_id -1).  A target outside 0 .. V - 1 makes its own
+ * row NaN.  A logit of -inf has probability 0; a row whose maximum is not finite has no
+ * distribution and is NaN, as log_softmax has it. */
+#define GHM_TOP_MAX 64        /* alternatives ghm_token_logprobs ranks per row */
+#define GHM_DISTILL_MAX 1024  /* teacher entries per row of ghm_distill */
+
+/* logprob[r] = log softmax(z_r)[targets[r]]; entropy[r] = - sum p log p; stats[r] =
+ * (max z, log sum exp(z - max)) for the backward; top_id / top_logprob [rows][top_k]:
+ * the top_k most likely values, descending, equal ones by ascending id (a NaN logit
+ * ranks first).  targets and logprob may be NULL together; entropy and stats may be
+ * NULL; top_k <= min(GHM_TOP_MAX, V). */
+int64_t ghm_token_logprobs_ws(int64_t rows, int64_t V, int top_k, int dtype);
+int ghm_token_logprobs(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner,
+                       int64_t rows, int64_t V, const void* targets, int id_bits, int64_t ignore_index, int top_k,
+                       float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_id, void* ws,
+                       int64_t ws_bytes, void* stream);
+/* dlogits [rows][V] (dtype, contiguous) from the gradients of logprob, entropy and
+ * top_logprob (each may be NULL), with the forward's stats, entropy and top_id. */
+int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner,
+                           int64_t rows, int64_t V, const void* targets, int id_bits, int64_t ignore_index,
+                           int top_k, const int64_t* top_id, const float* stats, const float* entropy,
+                           const float* d_logprob, const float* d_entropy, const float* d_top, void* dlogits,
+                           void* stream);
+
+/* Distillation from a teacher's top logits: top_ids / top_logits [rows][k] (entries
+ * with a negative id or a logit of -inf are absent; an id >= V makes its row NaN;
+ * repeated ids add up), q = softmax(top_logits / temperature) over a row's entries:
+ *   row_loss = (1 - alpha) CE(z, target) + alpha temperature^2 KL(q || softmax(z / temperature)).
+ * Counted rows: the target is not ignore_index; without targets (alpha = 1), at least
+ * one entry is present.  reduction 0: row_loss only; 1: loss[0] = mean over the counted
+ * rows (0 if there is none), norm[0] = 1 / their number; 2: loss[0] = sum.  stats
+ * [rows][4] for the backward.  dlogits non-NULL: also grad_scale * d(loss)/dz (reduction
+ * 0: of the sum) [rows][V], in the same call. */
+int64_t ghm_distill_ws(int64_t rows, int64_t V, int dtype);
+int ghm_distill(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner, int64_t rows,
+                int64_t V, const void* top_ids, int id_bits, const void* top_logits, int t_dtype, int k,
+                const void* targets, int target_bits, int64_t ignore_index, float temperature, float alpha,
+                int reduction, float* loss, float* row_loss, float* stats, float* norm, float grad_scale,
+                void* dlogits, void* ws, int64_t ws_bytes, void* stream);
+/* dlogits = d_loss * norm * d(sum of row losses)/dz; d_loss one value, or one per row
+ * (d_rows 1); norm NULL: 1. */
+int ghm_distill_bwd(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner, int64_t rows,
+                    int64_t V, const void* top_ids, int id_bits, const void* top_logits, int t_dtype, int k,
+                    const void* targets, int target_bits, int64_t ignore_index, float temperature, float alpha,
+                    const float* stats, const float* norm, const float* d_loss, int d_rows, void* dlogits,
+                    void* stream);
+
+/* out[i] = scale * weight[tokens[i]] (rows of D values, weight rows w_stride elements
+ * apart); a token outside 0 .. V - 1 gives a NaN row. */
+int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* weight, int dtype, int64_t w_stride, float scale,
+                       void* out, int64_t N, int64_t V, int64_t D, void* stream);
+/* dweight[v] = scale * sum_{i: tokens[i] = v} dout[i] [V][D], every row written: summed
+ * in f32 in the order of i over the sorted tokens and rounded once; row padding_idx
+ * (-1: none) is 0; tokens outside 0 .. V - 1 add nothing. */
+int64_t ghm_embed_rows_bwd_ws(int64_t N, int64_t V, int64_t D);
+int ghm_embed_rows_bwd(const void* tokens, int id_bits, const void* dout, int dtype, int64_t d_stride, float scale,
+                       int64_t padding_idx, void* dweight, int64_t N, int64_t V, int64_t D, void* ws,
+                       int64_t ws_bytes, void* stream);
+
 /* ---- helpers ----------------------------------------------------------- */
 /* number of 128-token blocks the token-parallel kernels use for M tokens */
 int64_t ghm_token_blocks(int64_t M);

@@ -144,13 +144,26 @@ HIP_SIGNATURES = {
     "ghm_scaled_diff": [_p, _p, _p, _f, _p, _i64, _p],
     "ghm_add_cols": [_p, _p, _i64, _i, _p],
     "ghm_adamw": [_p, _p, _p, _p, _i64, _p, _f, _f, _f, _f, _f, _p],
+    "ghm_token_logprobs_ws": [_i64, _i64, _i, _i],
+    "ghm_token_logprobs": [_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _i64, _i, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "ghm_token_logprobs_bwd": [_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _i64, _i, _p, _p, _p, _p, _p, _p, _p,
+                               _p],
+    "ghm_distill_ws": [_i64, _i64, _i],
+    "ghm_distill": [_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _i, _p, _i, _i64, _f, _f, _i, _p, _p, _p,
+                    _p, _f, _p, _p, _i64, _p],
+    "ghm_distill_bwd": [_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _i, _p, _i, _i64, _f, _f, _p, _p, _p,
+                        _i, _p, _p],
+    "ghm_embed_rows_fwd": [_p, _i, _p, _i, _i64, _f, _p, _i64, _i64, _i64, _p],
+    "ghm_embed_rows_bwd_ws": [_i64, _i64, _i64],
+    "ghm_embed_rows_bwd": [_p, _i, _p, _i, _i64, _f, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
     "ghm_zsc_logits": [_p, _i64, _p, _i, _p, _i, _i, _p, _i, _p, _p],
 }
 _RESTYPE = {"ghm_last_error_string": ctypes.c_char_p, "ghm_build_id": ctypes.c_char_p, "ghm_event_create": ctypes.c_void_p, "ghm_embed_bwd_part_elems": _i64, "ghm_embed_bwd_splits": _i, "ghm_guide_max_blocks": _i, "ghm_token_blocks": _i64,
             "ghm_mlp_bwd_rc_x3_blocks": _i64,
             "ghm_ln_rows_blocks": _i64, "ghm_gemm_slab_elems": _i64, "ghm_colsum_part_elems": _i64,
             "ghm_wcolsum_part_elems": _i64,
-            "ghm_ce_kl_out_elems": _i64}
+            "ghm_ce_kl_out_elems": _i64, "ghm_token_logprobs_ws": _i64, "ghm_distill_ws": _i64,
+            "ghm_embed_rows_bwd_ws": _i64}
 
 HOST_SIGNATURES = {
     "ghm_sampler_create": [_p, _p, _i, _i, _i, _i],

@@ -1,0 +1,660 @@
+"""The token operators (csrc/ghm_token.hip) against their definitions in 64 bits
+(oracle/token_oracle.py, which also gives the bound that a 32-bit evaluation with one
+final rounding may be off; the values below are never measured ones)."""
+import math
+
+import pytest
+import torch
+
+from oracle import token_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+    from ghmclip import _native
+    assert _native.hip_lib().ghm_device_ok() == 1
+
+
+def _M():
+    from ghmclip import models
+    return models
+
+
+def _near(got, want, bound, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in other places"
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]), f"{what}: infinities"
+    err, b = (got - want)[fin].abs(), bound[fin]
+    assert not torch.isnan(b).any(), what
+    bad = err > b
+    assert not bad.any(), f"{what}: off by {err[bad].max().item():.3e}, {(err[bad] / b[bad]).max().item():.2f} x the bound"
+
+
+def _grad_near(got, want, bound, dtype, what):
+    _near(got, want, bound * (1 + O.HALF[dtype]) + O.round_bound(want, dtype), what)
+
+
+def _logits(rows, V, dtype, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(rows, V, generator=g) * spread
+    z[torch.arange(rows), torch.randint(0, V, (rows,), generator=g)] += 7
+    return z.to(dtype)
+
+
+def _targets(rows, V, seed, ignored=True):
+    g = torch.Generator().manual_seed(seed + 1)
+    y = torch.randint(0, V, (rows,), generator=g)
+    if ignored and rows > 2:
+        y[rows // 2] = -100
+    return y
+
+
+def _check_score(z, y, k, got, what, ignore=-100):
+    """z on the CPU in its own type."""
+    r = O.score(z.double(), y, k, ignore)
+    if y is not None:
+        _near(got.logprob, r["logprob"], r["blogprob"], what + " logprob")
+    _near(got.entropy, r["entropy"], r["bentropy"], what + " entropy")
+    if k:
+        assert torch.equal(got.top_id.cpu(), r["top_id"]), what + " top_id"
+        _near(got.top_logprob, r["top_logprob"], r["btop_logprob"], what + " top_logprob")
+    return r
+
+
+SHAPES = [(1, 1), (3, 2), (5, 10), (513, 10), (7, 31), (7, 32), (7, 33), (4, 64), (3, 65), (66, 127), (2, 257), (9, 500),
+          (5, 1000), (2, 1024), (2, 2048), (2, 2049), (6, 3999), (3, 4097), (2, 8193), (1, 32771), (3, 70001), (300, 513),
+          (1, 200003)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", SHAPES)
+def test_score(rows, V, dtype):
+    M = _M()
+    z, y = _logits(rows, V, dtype, rows + V), _targets(rows, V, rows + V)
+    for k in sorted({0, 1, min(V, 5), min(V, 64)}):
+        got = M.token_logprobs(z.to(DEV), y.to(DEV), top_k=k)
+        assert got.logprob.dtype == got.entropy.dtype == torch.float32
+        _check_score(z, y, k, got, f"k {k}")
+        assert (got.top_id is None) == (k == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", SHAPES)
+def test_score_gradient(rows, V, dtype):
+    M = _M()
+    z, y = _logits(rows, V, dtype, rows + 3 * V), _targets(rows, V, V)
+    k = min(V, 7)
+    g = torch.Generator().manual_seed(5)
+    g1, g2, g3 = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.randn(rows, k, generator=g)
+    leaf = z.to(DEV).requires_grad_()
+    got = M.token_logprobs(leaf, y.to(DEV), top_k=k)
+    r = _check_score(z, y, k, got, "forward")
+    assert not got.top_id.requires_grad
+    both = (got.logprob * g1.to(DEV)).sum() + (got.entropy * g2.to(DEV)).sum() + (got.top_logprob * g3.to(DEV)).sum()
+    dz, = torch.autograd.grad(both, leaf, retain_graph=True)
+    want, bound = O.score_grad(z.double(), y, r, g1.double(), g2.double(), g3.double())
+    assert dz.dtype == dtype
+    _grad_near(dz, want, bound, dtype, "all three")
+    dz, = torch.autograd.grad(got.logprob, leaf, g1.to(DEV), retain_graph=True)
+    want, bound = O.score_grad(z.double(), y, r, g1.double())
+    _grad_near(dz, want, bound, dtype, "logprob alone")
+    dz, = torch.autograd.grad(got.top_logprob, leaf, g3.to(DEV))
+    want, bound = O.score_grad(z.double(), y, r, None, None, g3.double())
+    _grad_near(dz, want, bound, dtype, "alternatives alone")
+
+
+def test_score_gradient_against_differences():
+    M = _M()
+    z, y = _logits(3, 7, torch.float32, 2, 1.0), torch.tensor([1, 6, 3])
+    w = torch.randn(3, 2, generator=torch.Generator().manual_seed(3))
+
+    def f(x):
+        r = M.token_logprobs(x.to(DEV), y.to(DEV))
+        return torch.stack([r.logprob, r.entropy], -1).double().cpu()
+    leaf = z.to(DEV).requires_grad_()
+    r = M.token_logprobs(leaf, y.to(DEV))
+    dz, = torch.autograd.grad((r.logprob, r.entropy), leaf, (w[:, 0].to(DEV), w[:, 1].to(DEV)))
+    h = 2.0 ** -6
+    for v in range(7):
+        e = torch.zeros_like(z)
+        e[:, v] = h
+        num = ((f(z + e) - f(z - e)) / (2 * h) * w.double()).sum(-1)
+        # h^2 / 6 times a third derivative of at most 6 ln V, plus the rounding of two values over 2 h
+        tol = (h * h * math.log(7) + 2 * 32 * O.U / (2 * h) * 4) * w.double().abs().sum(-1)
+        assert ((dz[:, v].double().cpu() - num).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("V", [10, 300, 5000, 40000])
+@pytest.mark.parametrize("bits", [torch.uint8, torch.int32, torch.int64])
+def test_score_targets(V, bits):
+    """Padding rows are not read (NaN in them changes nothing), ids outside the
+    vocabulary poison their own row only."""
+    M = _M()
+    z, y = _logits(6, V, torch.float32, V), torch.tensor([3, 9, 200, 1, 0, 7])
+    ignore = 9
+    z[1] = math.nan
+    leaf = z.to(DEV).requires_grad_()
+    got = M.token_logprobs(leaf, y.to(bits).to(DEV), top_k=3, ignore_index=ignore)
+    _check_score(z, y, 3, got, "ids", ignore)
+    assert got.logprob[1] == 0 and got.entropy[1] == 0 and (got.top_id[1] == -1).all()
+    assert torch.isnan(got.logprob[2]).item() == (V == 10)
+    dz, = torch.autograd.grad(got.logprob.sum(), leaf)
+    assert (dz[1] == 0).all() and torch.isnan(dz[2]).all().item() == (V == 10)
+    assert torch.isfinite(dz[[0, 3, 4, 5]]).all()
+    if bits != torch.uint8:
+        got = M.token_logprobs(z.to(DEV), torch.tensor([-1, 9, V, 1, 0, 7], dtype=bits).to(DEV), ignore_index=ignore)
+        assert torch.isnan(got.logprob[[0, 2]]).all() and torch.isfinite(got.logprob[3:]).all()
+        assert torch.isfinite(got.entropy[[0, 2, 3]]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [10, 200, 3000, 9000])
+def test_score_masks_and_special_values(V, dtype):
+    M = _M()
+    z, y = _logits(10, V, dtype, V), torch.zeros(10, dtype=torch.long)
+    low = torch.finfo(dtype).min
+    z[0, 1:] = -math.inf                 # one value left
+    z[1, : V // 2] = -math.inf           # fewer values than alternatives in a part of the row
+    z[2, ::2] = low                      # the type's lowest value as a mask
+    z[3] = low                           # ... everywhere: uniform
+    z[4] = -math.inf                     # nothing left: no distribution
+    z[5, V - 1] = math.nan
+    z[6, 3] = math.inf
+    z[7] = 0.5                           # all equal
+    z[8] = torch.arange(V).to(dtype) / 16  # ascending: every step brings new alternatives
+    z[9] = torch.where(torch.arange(V) % 2 == 0, -0.0, 0.0)
+    k = min(V, 20)
+    leaf = z.to(DEV).requires_grad_()
+    got = M.token_logprobs(leaf, y.to(DEV), top_k=k)
+    r = _check_score(z, y, k, got, "special")
+    dz, = torch.autograd.grad((got.logprob.sum() + got.entropy.sum()), leaf)
+    one = torch.ones(10, dtype=torch.float64)
+    want, bound = O.score_grad(z.double(), y, r, one, one)
+    rows = [0, 1, 2, 3, 7, 8, 9]
+    _grad_near(dz[rows], want[rows], bound[rows], dtype, "gradient")
+    assert torch.isnan(dz[[4, 5, 6]]).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [50, 700, 20000])
+def test_score_ties(V, dtype):
+    """Few distinct values: the alternatives are the lowest ids of the largest values."""
+    M = _M()
+    g = torch.Generator().manual_seed(V)
+    z = torch.randint(-3, 4, (9, V), generator=g).to(dtype)
+    z[3] = -z[3].abs()
+    z[4, V // 3:] = 3
+    z[5] = torch.arange(V, 0, -1).to(dtype)
+    for k in (1, 5, 33, 50):
+        got = M.token_logprobs(z.to(DEV), top_k=k)
+        assert got.logprob is None
+        _check_score(z, None, k, got, f"ties k {k}")
+
+
+def test_score_views():
+    """Rows read in place past a prefix, every second row, values of a wider row, shifted
+    storage, transposed and expanded logits; leading dimensions kept."""
+    M = _M()
+    g = torch.Generator().manual_seed(9)
+    for dtype in DTYPES:
+        base = (torch.randn(4, 6, 37, generator=g) * 2).to(dtype)
+        for make in (lambda x: x[:, 1:], lambda x: x[::2], lambda x: x[..., 3:20], lambda x: x[0, 0],
+                     lambda x: x.transpose(1, 2), lambda x: x[:1].expand(3, -1, -1), lambda x: x[1:, 2:4, 5:],
+                     lambda x: x[:, :1, :1], lambda x: x[:0]):
+            z = make(base)
+            lead, V = z.shape[:-1], z.shape[-1]
+            y = torch.randint(0, V, lead, generator=g)
+            k = min(V, 4)
+            on = make(base.to(DEV)).detach().requires_grad_()
+            got = M.token_logprobs(on, y.to(DEV), top_k=k)
+            assert got.logprob.shape == got.entropy.shape == lead and got.top_id.shape == (*lead, k)
+            flat = M.TokenScores(got.logprob.reshape(-1), got.entropy.reshape(-1), got.top_logprob.reshape(-1, k),
+                                 got.top_id.reshape(-1, k))
+            if z.numel() == 0:
+                continue
+            r = _check_score(z.reshape(-1, V), y.reshape(-1), k, flat, "view")
+            dz, = torch.autograd.grad(got.logprob.sum(), on)
+            want, bound = O.score_grad(z.reshape(-1, V).double(), y.reshape(-1), r, torch.ones(max(1, y.numel())).double())
+            assert dz.shape == z.shape
+            _grad_near(dz.reshape(-1, V), want, bound, dtype, "view gradient")
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^31 elements apart, in and out of every operator."""
+    M = _M()
+    V, step = 1000, 1 << 31
+    buf = torch.empty(2 * step + V + 8, dtype=torch.bfloat16, device=DEV)
+    z = torch.as_strided(buf, (3, V), (step, 1), 3)
+    zc, y = _logits(3, V, torch.bfloat16, 1), torch.tensor([5, 999, 0])
+    z.copy_(zc)
+    _check_score(zc, y, 4, M.token_logprobs(z, y.to(DEV), top_k=4), "far rows")
+    ids, t = torch.tensor([[1, 2], [3, 4], [999, 0]]), torch.randn(3, 2)
+    loss, dz = M.distill_loss_and_grad(z, ids.to(DEV), t.to(DEV), reduction="sum")
+    r = O.distill(zc.double(), ids, t.double(), None, 1.0, 1.0)
+    _near(loss, r["row_loss"].sum(), r["brow_loss"].sum() + 8 * O.U * r["row_loss"].abs().sum(), "far loss")
+    _grad_near(dz, r["dz"], r["bdz"], torch.bfloat16, "far gradient")
+    del buf, z
+    D = 4096  # a table of more than 2^32 elements
+    V = (1 << 20) + 3
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device=DEV)
+    tok = torch.tensor([V - 1, 5, V - 1, 1 << 20, 524288])
+    rows = torch.randn(5, D).to(torch.bfloat16)
+    w[tok] = rows[[2, 1, 2, 3, 4]].to(DEV)
+    w.requires_grad_()
+    out = M.scaled_embedding(tok.to(DEV), w, 2.0)
+    assert torch.equal(out.detach().cpu(), rows[[2, 1, 2, 3, 4]] * 2)
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert dw[V - 1].eq(4).all() and dw[5].eq(2).all() and dw[1 << 20].eq(2).all() and dw[524288].eq(2).all()
+    assert int(dw.ne(0).any(-1).sum()) == 4
+
+
+# ---- distillation ---------------------------------------------------------
+
+
+def _teacher(rows, V, k, seed, ragged=True):
+    g = torch.Generator().manual_seed(seed + 7)
+    ids = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(rows)])
+    t = torch.randn(rows, k, generator=g) * 2
+    if ragged and rows > 3:
+        ids[1] = -1                      # no entry at all
+        ids[2, k // 2:] = -1
+        t[3, 0] = -math.inf
+    return ids, t
+
+
+def _check_distill(z, ids, t, y, tau, alpha, dtype, what):
+    M = _M()
+    r = O.distill(z.double(), ids, t.double(), y, tau, alpha)
+    on = [z.to(DEV), ids.to(DEV), t.to(DEV), None if y is None else y.to(DEV)]
+    opts = dict(temperature=tau, alpha=alpha)
+    rows = M.distill_loss(*on, reduction="none", **opts)
+    assert rows.dtype == torch.float32
+    _near(rows, r["row_loss"], r["brow_loss"], what + " rows")
+    n = max(1, int(r["counted"].sum()))
+    total, btotal = r["row_loss"].sum(), r["brow_loss"].sum() + (len(z) + 24) * O.U * r["row_loss"].abs().sum()
+    loss, dz = M.distill_loss_and_grad(*on, **opts)
+    _near(loss, total / n, btotal / n + 4 * O.U * total.abs() / n, what + " mean")
+    _grad_near(dz, r["dz"] / n, (r["bdz"] + 4 * O.U * r["dz"].abs()) / n, dtype, what + " step gradient")
+    leaf = on[0].clone().requires_grad_()
+    loss = M.distill_loss(leaf, *on[1:], reduction="sum", **opts)
+    _near(loss, total, btotal, what + " sum")
+    got, = torch.autograd.grad(loss * 3, leaf)
+    _grad_near(got, 3 * r["dz"], 3 * (r["bdz"] + 4 * O.U * r["dz"].abs()), dtype, what + " autograd")
+    up = torch.linspace(-1, 2, len(z), dtype=torch.float64)
+    got, = torch.autograd.grad(M.distill_loss(leaf, *on[1:], reduction="none", **opts), leaf, up.float().to(DEV))
+    u32 = up.float().double()[:, None]
+    _grad_near(got, u32 * r["dz"], (r["bdz"] + 4 * O.U * r["dz"].abs()) * u32.abs(), dtype, what + " rows' autograd")
+    return loss
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", SHAPES)
+def test_distill(rows, V, dtype):
+    z, y = _logits(rows, V, dtype, rows + V), _targets(rows, V, V + 2)
+    for k, tau, alpha in ((min(V, 4), 1.0, 1.0), (min(V, 17), 2.0, 1.0), (min(V, 64), 1.0, 0.5), (min(V, 5), 3.0, 0.25),
+                          (1, 0.5, 0.0)):
+        ids, t = _teacher(rows, V, k, rows + V)
+        _check_distill(z, ids, t, y if alpha < 1 or k == 1 else None, tau, alpha, dtype, f"k {k} tau {tau} alpha {alpha}")
+
+
+@pytest.mark.parametrize("V", [10, 40, 3000, 20000])
+@pytest.mark.parametrize("k", [1, 3, 1000, 1024])
+def test_distill_entries(V, k):
+    """More entries than values, repeated ids, teacher logits of 16 bits, 32-bit ids."""
+    g = torch.Generator().manual_seed(V + k)
+    z = _logits(6, V, torch.float32, V)
+    ids = torch.randint(0, V, (6, k), generator=g).int()
+    t = torch.randn(6, k, generator=g).to(torch.bfloat16)
+    if k > 1:
+        ids[1] = ids[1, 0]
+        ids[2, 1] = -5
+    y = _targets(6, V, 1)
+    _check_distill(z, ids.long(), t.float(), None, 2.0, 1.0, torch.float32, "entries")
+    M = _M()
+    a = M.distill_loss_and_grad(z.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV).int(), temperature=2.0, alpha=0.5)
+    b = M.distill_loss_and_grad(z.to(DEV), ids.long().to(DEV), t.float().to(DEV), y.to(DEV), temperature=2.0, alpha=0.5)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("V", [10, 300, 3000, 20000])
+def test_distill_special_values(V):
+    M = _M()
+    z = _logits(8, V, torch.float32, V)
+    ids, t = _teacher(8, V, 4, V, ragged=False)
+    y = torch.full((8,), 2)
+    y[7] = -100
+    z[0, :] = -math.inf
+    z[0, ids[0]] = 1.0                   # only the teacher's values are left
+    z[0, 2] = 0.0
+    z[1, ids[1, 1]] = -math.inf          # the student rules out a value the teacher holds: infinite loss
+    z[7] = math.nan                      # padding: not read
+    t[7] = math.nan
+    r = O.distill(z[:2].double(), ids[:2], t[:2].double(), None, 1.0, 1.0)
+    rows = M.distill_loss(z[:2].to(DEV), ids[:2].to(DEV), t[:2].to(DEV), reduction="none")
+    _near(rows, r["row_loss"], r["brow_loss"].nan_to_num(0, 0), "ruled out")
+    assert rows[1] == math.inf
+    ids[2, 0] = V                        # an id outside the vocabulary
+    y[3] = V + 5
+    t[4, 1] = math.nan
+    t[5, 1] = math.inf
+    for tau, alpha in ((1.0, 0.5), (2.0, 0.5)):
+        loss, dz = M.distill_loss_and_grad(z.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV), temperature=tau, alpha=alpha,
+                                           reduction="none")
+        assert torch.isnan(loss[2:6]).all() and torch.isfinite(loss[[0, 6, 7]]).all()
+        assert torch.isnan(dz[2:6]).any(-1).all() and torch.isfinite(dz[[0, 1, 6, 7]]).all() and (dz[7] == 0).all()
+
+
+def test_distill_nothing_counts():
+    M = _M()
+    z = _logits(5, 77, torch.float32, 0).to(DEV).requires_grad_()
+    ids, t = torch.full((5, 3), -1, device=DEV), torch.zeros(5, 3, device=DEV)
+    loss = M.distill_loss(z, ids, t)
+    dz, = torch.autograd.grad(loss, z)
+    assert loss == 0 and (dz == 0).all()
+    y = torch.full((5,), -100, device=DEV)
+    loss, dz = M.distill_loss_and_grad(z.detach(), ids, t, y, alpha=0.5)
+    assert loss == 0 and (dz == 0).all()
+    loss, dz = M.distill_loss_and_grad(z.detach()[:0], ids[:0], t[:0])
+    assert loss == 0 and dz.shape == (0, 77)
+    assert M.distill_loss(z.detach()[:0], ids[:0], t[:0], reduction="none").shape == (0,)
+
+
+def test_distill_views_and_module():
+    M = _M()
+    base = _logits(24, 37, torch.bfloat16, 3).view(4, 6, 37)
+    ids, t = _teacher(20, 37, 5, 1)
+    z = base.to(DEV)[:, 1:]
+    r = O.distill(base[:, 1:].reshape(20, 37).double(), ids, t.double(), None, 2.0, 1.0)
+    leaf = z.detach().requires_grad_()
+    loss = M.TopLogitsDistillLoss(temperature=2.0, reduction="sum")(leaf, ids.view(4, 5, 5).to(DEV), t.view(4, 5, 5).to(DEV))
+    loss.backward()
+    _near(loss, r["row_loss"].sum(), r["brow_loss"].sum() + 44 * O.U * r["row_loss"].abs().sum(), "view loss")
+    _grad_near(leaf.grad.reshape(20, 37), r["dz"], r["bdz"] + 4 * O.U * r["dz"].abs(), torch.bfloat16, "view gradient")
+
+
+def test_distill_gradient_against_differences():
+    M = _M()
+    z, y = _logits(3, 7, torch.float32, 2, 1.0), torch.tensor([1, 6, 3])
+    ids, t = torch.tensor([[0, 3], [6, 2], [5, -1]]), torch.tensor([[1.0, 0.5], [2.0, -1.0], [0.3, 9.0]])
+    opts = dict(temperature=2.0, alpha=0.5)
+
+    def f(x):
+        return M.distill_loss(x.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV), reduction="none", **opts).double().cpu()
+    _, dz = M.distill_loss_and_grad(z.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV), reduction="sum", **opts)
+    h = 2.0 ** -6
+    for v in range(7):
+        e = torch.zeros_like(z)
+        e[:, v] = h
+        num = (f(z + e) - f(z - e)) / (2 * h)
+        # third derivatives of the two log-sum-exps: at most 1 and 1 / tau
+        assert ((dz[:, v].double().cpu() - num).abs() <= h * h + 2 * 64 * O.U * 8 / (2 * h)).all()
+
+
+# ---- embedding ------------------------------------------------------------
+
+EMBED_SHAPES = [(1, 1, 1), (1, 10, 256), (7, 3, 5), (64, 10, 64), (1000, 10, 33), (513, 257, 128), (4096, 50, 8),
+                (3000, 70001, 16), (9000, 300, 96), (20000, 7, 130), (40000, 1000, 40), (33, 5, 4096), (70000, 2, 8)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,D", EMBED_SHAPES)
+def test_embedding(N, V, D, dtype):
+    M = _M()
+    g = torch.Generator().manual_seed(N + V + D)
+    tok = (torch.rand(N, generator=g) ** 3 * V).long().clamp(max=V - 1)
+    w = torch.randn(V, D, generator=g).to(dtype)
+    dout = torch.randn(N, D, generator=g).to(dtype)
+    scale = float(torch.tensor(math.sqrt(D)))
+    for pad in (None, V - 1):
+        leaf = w.to(DEV).requires_grad_()
+        out = M.scaled_embedding(tok.to(DEV), leaf, scale, padding_idx=pad)
+        want, bound = O.embed(tok, w.double(), scale)
+        assert out.dtype == dtype
+        _grad_near(out, want, bound, dtype, "rows")
+        dw, = torch.autograd.grad(out, leaf, dout.to(DEV))
+        want, bound = O.embed_grad(tok, dout.double(), scale, V, pad)
+        _grad_near(dw, want, bound, dtype, "gradient")
+        again, = torch.autograd.grad(M.scaled_embedding(tok.to(DEV), leaf, scale, padding_idx=pad), leaf, dout.to(DEV))
+        assert torch.equal(dw, again)
+
+
+@pytest.mark.parametrize("bits", [torch.uint8, torch.int32, torch.int64])
+@pytest.mark.parametrize("N", [5, 3000, 30000])
+def test_embedding_tokens(N, bits):
+    """Tokens of every width and outside the table, one token repeated, none of a range,
+    shapes of any rank, strided tables and gradients."""
+    M = _M()
+    g = torch.Generator().manual_seed(N)
+    V, D = 200, 24
+    tok = torch.randint(0, 256 if bits == torch.uint8 else 230, (N,), generator=g)
+    if bits != torch.uint8:
+        tok[0], tok[-1] = -1, V
+    w, dout = torch.randn(V, 2 * D, generator=g), torch.randn(N, D + 7, generator=g)
+    leaf = w.to(DEV)[:, :D].detach().requires_grad_()
+    out = M.scaled_embedding(tok.to(bits).to(DEV), leaf, 0.5)
+    want, bound = O.embed(tok, w[:, :D].double(), 0.5)
+    _grad_near(out, want, bound, torch.float32, "rows")
+    dw, = torch.autograd.grad(out, leaf, dout.to(DEV)[:, :D])
+    want, bound = O.embed_grad(tok, dout[:, :D].double(), 0.5, V)
+    _grad_near(dw, want, bound, torch.float32, "gradient")
+    one = torch.full((N,), 3, dtype=bits, device=DEV).view(-1, 5 if N % 5 == 0 else 1)
+    out = M.scaled_embedding(one, leaf, 1.0)
+    assert out.shape == (*one.shape, D)
+    dw, = torch.autograd.grad(out.sum(), leaf)  # an expanded gradient
+    assert (dw[3] == N).all() and int(dw.ne(0).any(-1).sum()) == 1
+    dw, = torch.autograd.grad(M.scaled_embedding(one[:0], leaf), leaf, torch.zeros(0, one.shape[1], D, device=DEV))
+    assert (dw == 0).all()
+
+
+def test_embedding_module():
+    M = _M()
+    torch.manual_seed(0)
+    ref = torch.nn.Embedding(50, 12, padding_idx=-1)
+    torch.manual_seed(0)
+    emb = M.ScaledEmbedding(50, 12, padding_idx=-1, scale=3.0).to(DEV)
+    assert torch.equal(ref.weight, emb.weight.cpu())
+    tok = torch.tensor([[1, 49, 3], [1, 1, 0]])
+    emb(tok.to(DEV)).sum().backward()
+    assert emb.weight.grad[1].eq(9).all() and emb.weight.grad[49].eq(0).all() and emb.weight.grad[2].eq(0).all()
+
+
+# ---- how they are called --------------------------------------------------
+
+
+def test_refusals():
+    M = _M()
+    z = torch.zeros(4, 10, device=DEV)
+    y = torch.zeros(4, dtype=torch.long, device=DEV)
+    with pytest.raises(TypeError, match="float32"):
+        M.token_logprobs(z.double(), y)
+    with pytest.raises(TypeError, match="targets"):
+        M.token_logprobs(z, y.float())
+    with pytest.raises(ValueError, match="targets"):
+        M.token_logprobs(z, y[:3])
+    with pytest.raises(ValueError, match="targets"):
+        M.token_logprobs(z, y.cpu())
+    for k in (-1, 11, 65, 2.0):
+        with pytest.raises(ValueError, match="top_k"):
+            M.token_logprobs(z, y, top_k=k)
+    with pytest.raises(ValueError, match="V >= 1"):
+        M.token_logprobs(z[:, :0])
+    ids, t = torch.zeros(4, 2, dtype=torch.long, device=DEV), torch.zeros(4, 2, device=DEV)
+    for bad in (dict(temperature=0.0), dict(temperature=math.inf), dict(temperature=math.nan), dict(alpha=0.5),
+                dict(alpha=-0.1), dict(alpha=1.1), dict(reduction="median")):
+        with pytest.raises(ValueError):
+            M.distill_loss(z, ids, t, **bad)
+    with pytest.raises(TypeError, match="top_ids"):
+        M.distill_loss(z, ids.to(torch.uint8), t)
+    with pytest.raises(ValueError, match="top_ids"):
+        M.distill_loss(z, ids[:3], t)
+    with pytest.raises(ValueError, match="top_ids"):
+        M.distill_loss(z, ids[:, :0], t[:, :0])
+    with pytest.raises(ValueError, match="top_logits"):
+        M.distill_loss(z, ids, t[:, :1])
+    with pytest.raises(TypeError, match="top_logits"):
+        M.distill_loss(z, ids, t.double())
+    w = torch.zeros(10, 4, device=DEV)
+    with pytest.raises(TypeError, match="weight"):
+        M.scaled_embedding(y, w.double())
+    with pytest.raises(TypeError, match="tokens"):
+        M.scaled_embedding(y.float(), w)
+    with pytest.raises(ValueError, match="weight"):
+        M.scaled_embedding(y, w[0])
+    for pad in (10, -11):
+        with pytest.raises(ValueError, match="padding_idx"):
+            M.scaled_embedding(y, w, padding_idx=pad)
+
+
+def test_second_gradient_is_refused():
+    M = _M()
+    z = torch.randn(3, 9, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(M.token_logprobs(z, torch.zeros(3, dtype=torch.long, device=DEV)).logprob.sum(), z,
+                             create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def _calls(z, y, ids, t, w, tok):
+    """One run of each operator with its gradient; all outputs."""
+    M = _M()
+    r = M.token_logprobs(z, y, top_k=5)
+    a, = torch.autograd.grad((r.logprob, r.entropy), z, (torch.ones_like(r.logprob), torch.ones_like(r.entropy)))
+    loss = M.distill_loss(z, ids, t, y, temperature=2.0, alpha=0.5)
+    b, = torch.autograd.grad(loss, z)
+    c = M.distill_loss_and_grad(z.detach(), ids, t)
+    out = M.scaled_embedding(tok, w, 2.0)
+    d, = torch.autograd.grad(out, w, torch.ones_like(out))
+    return [r.logprob, r.entropy, r.top_logprob, r.top_id, a, loss, b, *c, out, d]
+
+
+def _inputs(rows, V, seed, dtype=torch.float32):
+    z = _logits(rows, V, dtype, seed).to(DEV).requires_grad_()
+    ids, t = _teacher(rows, V, 4, seed)
+    g = torch.Generator().manual_seed(seed)
+    return [z, _targets(rows, V, seed).to(DEV), ids.to(DEV), t.to(DEV),
+            torch.randn(V, 16, generator=g).to(DEV).requires_grad_(), torch.randint(0, V, (3 * rows,), generator=g).to(DEV)]
+
+
+@pytest.mark.parametrize("rows,V", [(40, 10), (3, 40000), (700, 3000)])
+def test_captured_and_replayed(rows, V):
+    """Two graphs and eager calls in turn: every replay has the eager bits."""
+    sets = [_inputs(rows, V, s) for s in (1, 2)]
+    other = _inputs(rows, V, 3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(s):
+        for x in sets:
+            _calls(*x)
+        for x in sets:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                outs.append([o.detach() for o in _calls(*x)])
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(s)
+    want = [o.detach().clone() for o in _calls(*other)]
+    for turn in range(3):
+        with torch.no_grad():
+            for x, k in zip(sets, (0, 1)):
+                x[0].copy_(_logits(rows, V, torch.float32, 10 * turn + k))
+        graphs[0].replay()
+        graphs[1].replay()
+        mine = [o.detach() for o in _calls(*other)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(mine, want))
+        for x, got in zip(sets, outs):
+            assert all(torch.equal(a, b.detach()) for a, b in zip(got, _calls(*x)))
+
+
+def test_other_streams():
+    """Calls on two streams at once, each on its own inputs, have the bits of calls alone."""
+    sets = [_inputs(300, 9000, s, torch.bfloat16) for s in (1, 2)]
+    for x in sets:
+        x[4] = x[4].detach().requires_grad_()
+    want = [[o.detach().clone() for o in _calls(*x)] for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append([o.detach() for o in _calls(*x)])
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_distilling_the_vlm():
+    """A run of the operators as they are used: the teacher's next-token logits scored,
+    their alternatives kept, a student's model trained on them; its parameters' gradients
+    equal those of the same loss written in torch operations."""
+    M = _M()
+    torch.manual_seed(0)
+    B, T1, V = 4, 12, 10
+    kw = dict(n_token=T1 + 1, n_i_token=1, num_class=V, n_embd=128, n_guided_layers=[1, 1], n_mlp_hidden=512,
+              auto_regressive=True, sequential=True, layernorm=True)
+    teacher, student = (M.AutoRegressiveTransformer(n_layer=n, **kw).to(DEV) for n in (4, 3))
+    xt, zi = torch.randint(0, V, (B, T1), device=DEV), torch.randn(B, 1, V, device=DEV)
+    y = torch.randint(0, V, (B, T1), device=DEV)
+    y[0, :3] = -100
+    with torch.no_grad():
+        s = M.token_logprobs(teacher(xt, zi)[0], y, top_k=4)
+    live = y != -100
+    assert (s.top_id[~live] == -1).all() and (s.top_id[live] >= 0).all()
+    loss_fn = M.TopLogitsDistillLoss(temperature=2.0, alpha=0.7)
+    logits = student(xt, zi)[0]
+    loss = loss_fn(logits, s.top_id, s.top_logprob, y)
+    loss.backward()
+    got = {n: p.grad.clone() for n, p in student.named_parameters() if p.grad is not None}
+    student.zero_grad()
+    logits = student(xt, zi)[0]
+    z = logits.double()
+    q = torch.softmax(s.top_logprob.double() / 2, -1)
+    kl = (q * (q.log() - torch.log_softmax(z / 2, -1).gather(-1, s.top_id.clamp(min=0)))).sum(-1)
+    ce = -torch.log_softmax(z, -1).gather(-1, y.clamp(min=0)[..., None])[..., 0]
+    want = ((0.3 * ce + 0.7 * 4 * kl) * live).sum() / live.sum()
+    want.backward()
+    assert abs(loss.item() - want.item()) <= 64 * O.U * abs(want.item())
+    assert got
+    for n, p in student.named_parameters():
+        if n in got:
+            # the same backward kernels on logits gradients that differ by f32 rounding; the
+            # largest entry carries the scale through the layers
+            assert (got[n] - p.grad).abs().max() <= 1e-4 * p.grad.abs().max() + 1e-9, n
+
+
+def test_both_ends_of_a_vocabulary():
+    """Scaled embedding, tied readout, distillation and scoring together on a vocabulary
+    of 3,001 values: the table's gradient from both ends against 64 bits."""
+    M = _M()
+    V, D, B, T = 3001, 32, 3, 11
+    g = torch.Generator().manual_seed(4)
+    emb = M.ScaledEmbedding(V, D, scale=math.sqrt(D)).to(DEV)
+    tok = torch.randint(0, V, (B, T), generator=g)
+    tlog = torch.randn(B, T, V, generator=g) * 3
+    s = M.token_logprobs(tlog.to(DEV), top_k=8)
+    h = emb(tok.to(DEV))
+    logits = h @ emb.weight.t()
+    loss = M.distill_loss(logits, s.top_id, s.top_logprob, temperature=2.0)
+    loss = loss - 0.01 * M.token_logprobs(logits).entropy.mean()
+    loss.backward()
+    w = emb.weight.detach().double().cpu().requires_grad_()
+    z = (w[tok] * emb.scale) @ w.t()
+    q = torch.softmax(s.top_logprob.double().cpu() / 2, -1)
+    kl = 4 * (q * (q.log() - torch.log_softmax(z / 2, -1).gather(-1, s.top_id.cpu()))).sum(-1).mean()
+    p = torch.softmax(z, -1)
+    want = kl + 0.01 * (p * torch.log_softmax(z, -1)).sum(-1).mean()
+    want.backward()
+    assert abs(loss.item() - want.item()) <= 1e-5 * abs(want.item())
+    # f32 products over D and V terms on both sides of the operators
+    assert (emb.weight.grad.double().cpu() - w.grad).abs().max() <= 1e-5 * w.grad.abs().max()
