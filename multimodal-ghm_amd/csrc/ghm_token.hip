@@ -60,6 +60,343 @@ __device__ __forceinline__ uint64_t top_key(float x, uint32_t id) {
   return (static_cast<uint64_t>(order_bits(x)) << 32) | (0xffffffffu - id);
 }
 
+// 16 bytes of a row as floats, and back, at any element alignment
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+template <typename T>
+struct Vec {
+  static constexpr int N = 8;
+  using raw = u32x4_a2;
+};
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  using raw = u32x4_a4;
+};
+template <int N, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
+  if constexpr (N == 1) {
+    x[0] = to_f(*p);
+  } else {
+    static_assert(N == Vec<T>::N, "one value or 16 bytes");
+    const u32x4 v = *reinterpret_cast<const typename Vec<T>::raw*>(p);
+    T e[N];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f(e[i]);
+  }
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+  if constexpr (N == 1) {
+    from_f(*p, x[0]);
+  } else {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) from_f(e[i], x[i]);
+    u32x4 v;
+    __builtin_memcpy(&v, e, 16);
+    *reinterpret_cast<typename Vec<T>::raw*>(p) = v;
+  }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ void wave_fence() {  // this wave's LDS writes before its later reads
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A group of W waves works on one row (W == 1: no barrier, the block holds several).
+// Reductions go through slots of LDS in a fixed order; every use names a slot of its own.
+template <int W>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (W > 1) __syncthreads();
+  else wave_fence();
+}
+template <int W>
+__device__ __forceinline__ float group_max(float v, float* slot, int w) {
+  v = wave_max(v);
+  if constexpr (W == 1) return v;
+  if ((threadIdx.x & 63) == 0) slot[w] = v;
+  __syncthreads();
+  v = slot[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) v = fmaxf(v, slot[i]);
+  return v;
+}
+template <int W>
+__device__ __forceinline__ float group_sum(float v, float* slot, int w) {
+  v = wave_sum(v);
+  if constexpr (W == 1) return v;
+  if ((threadIdx.x & 63) == 0) slot[w] = v;
+  __syncthreads();
+  v = slot[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) v += slot[i];
+  return v;
+}
+
+// One pass over a row: a lane's running maximum m and sums relative to it.
+//   s = sum e^{c1 (z - m)};  SECOND_ENT: t = sum e^{c1 d} d (d = z - m);
+//   SECOND_EXP: t = sum e^{c2 d};  SECOND_NONE: t unused.
+// The maximum starts at the lowest finite value, so differences never are -inf minus
+// -inf; a difference is cut at -1e4 where it is a factor (e^-1e4 = 0).  NaN and +inf
+// make s NaN.  c1, c2 carry log2 e.
+enum { SECOND_NONE, SECOND_ENT, SECOND_EXP };
+struct Sums {
+  float m = -FLT_MAX, s = 0.f, t = 0.f;
+};
+template <int SECOND>
+__device__ __forceinline__ void rebase(Sums& a, float m, float c1, float c2) {
+  const float dm = fmaxf(a.m - m, -1e4f), f = __builtin_amdgcn_exp2f(dm * c1);
+  if constexpr (SECOND == SECOND_ENT) a.t = f * (a.t + dm * a.s);
+  if constexpr (SECOND == SECOND_EXP) a.t *= __builtin_amdgcn_exp2f(dm * c2);
+  a.s *= f;
+  a.m = m;
+}
+template <int SECOND, int N>
+__device__ __forceinline__ void fold(Sums& a, const float (&x)[N], float c1, float c2) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - a.m, e = __builtin_amdgcn_exp2f(d * c1);
+    a.s += e;
+    if constexpr (SECOND == SECOND_ENT) a.t += e * fmaxf(d, -1e4f);
+    if constexpr (SECOND == SECOND_EXP) a.t += __builtin_amdgcn_exp2f(d * c2);
+  }
+}
+// the group's sums in every lane
+template <int SECOND, int W>
+__device__ __forceinline__ Sums group_join(Sums a, float* slots, int w, float c1, float c2) {
+  rebase<SECOND>(a, group_max<W>(a.m, slots, w), c1, c2);
+  a.s = wave_sum(a.s);
+  if constexpr (SECOND != SECOND_NONE) a.t = wave_sum(a.t);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) {
+      slots[W + w] = a.s;
+      if constexpr (SECOND != SECOND_NONE) slots[2 * W + w] = a.t;
+    }
+    __syncthreads();
+    a.s = slots[W];
+#pragma unroll
+    for (int i = 1; i < W; ++i) a.s += slots[W + i];
+    if constexpr (SECOND != SECOND_NONE) {
+      a.t = slots[2 * W];
+#pragma unroll
+      for (int i = 1; i < W; ++i) a.t += slots[2 * W + i];
+    }
+  }
+  return a;
+}
+
+// ---- the largest values of a row, found in the same pass -------------------
+// Each wave keeps candidates (64-bit keys) in LDS: the values above a threshold that
+// only rises.  Valid thresholds: (a) with r = ceil(k / W), the least over the waves of
+// each wave's r-th largest lane maximum: the waves hold k values at or above it;
+// (b) a wave's own k-th candidate after a prune, strictly, for its later (higher) ids.
+// A few hundred of a row's values become candidates; the k best of them are ranked at
+// the end by counting.
+constexpr int TOP_CAP = 576;  // 64 kept by a prune + one vector of 8 values per lane
+
+// at least r lanes hold u >= the result (its upper 16 bits are searched: a lower bound
+// of the r-th largest); 0: fewer
+__device__ __forceinline__ uint32_t kth_bits(uint32_t u, int r) {
+  uint32_t K = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t c = K | (1u << b);
+    if (__popcll(__ballot(u >= c)) >= r) K = c;
+  }
+  return K;
+}
+// the float just below order bits K: x > it is order_bits(x) >= K.  NaN (nothing is at
+// or below it) if K is no more than what a lane without values holds.
+__device__ __forceinline__ float below(uint32_t K) {
+  if (K <= 0x00800000u) return __builtin_nanf("");
+  const uint32_t o = K - (K == 0x80000000u ? 2 : 1);  // -0 is equal to +0, not below it
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+
+// keep the k largest of a wave's n candidates, in descending order
+__device__ __forceinline__ void top_prune(uint64_t* cand, int n, int k, int lane) {
+  constexpr int M = TOP_CAP / 64;
+  uint64_t mine[M];
+  int rank[M];
+  wave_fence();
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    mine[j] = lane + 64 * j < n ? cand[lane + 64 * j] : 0;
+    rank[j] = 0;
+  }
+  for (int i = 0; i < n; ++i) {
+    const uint64_t c = cand[i];
+#pragma unroll
+    for (int j = 0; j < M; ++j) rank[j] += c > mine[j];
+  }
+  wave_fence();
+#pragma unroll
+  for (int j = 0; j < M; ++j)
+    if (lane + 64 * j < n && rank[j] < k) cand[rank[j]] = mine[j];
+  wave_fence();
+}
+
+// A row's values lo .. hi - 1, lane by lane: batches of U vectors of N values; the
+// values after the last whole vector go to wave 0.  Vectors and batches of a wave come
+// in ascending order.  TOP: k candidates are kept in cand (n of them on return), thr
+// and the shared lane-maximum bounds tw as above.
+template <typename T, int N, int U, int W, int SECOND, bool TOP>
+__device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, float c2, int w, int lane, int k,
+                                         uint64_t* cand, uint32_t* tw, int& n_cand, uint32_t& bound) {
+  Sums a;
+  float thr = __builtin_nanf("");
+  int cnt = 0;
+  const int nv = (hi - lo) / N, tail = (hi - lo) - nv * N;
+  const int r = TOP ? (k + W - 1) / W : 0;
+  constexpr int STEP = W * 64 * U;
+  const int nb = (nv + STEP - 1) / STEP + (tail && N > 1 ? 1 : 0);  // the tail is one batch of its own
+  const int full = (nv + STEP - 1) / STEP;
+  for (int b = 0; b < nb; ++b) {
+    float x[U][N], vm[U];
+    bool valid[U];
+    const bool is_tail = b == full;
+    const int v0 = b * STEP + w * 64 + lane;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      valid[u] = !is_tail && v0 + u * W * 64 < nv;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = NEG_INF;
+      if (valid[u]) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
+    }
+    if (is_tail) {
+      valid[0] = w == 0 && lane < tail;
+      if (valid[0]) x[0][0] = to_f(z[lo + nv * N + lane]);
+    }
+    float bm = -FLT_MAX;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      vm[u] = x[u][0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) vm[u] = fmaxf(vm[u], x[u][i]);
+      bm = fmaxf(bm, vm[u]);
+    }
+    rebase<SECOND>(a, fmaxf(a.m, bm), c1, c2);
+#pragma unroll
+    for (int u = 0; u < U; ++u) fold<SECOND>(a, x[u], c1, c2);
+    if constexpr (TOP) {
+      // refresh the shared bound after batches 1, 2, 4, 8, ... and the last
+      if (((b + 1) & b) == 0 || b == nb - 1) {
+        const uint32_t K = kth_bits(order_bits(a.m), r);
+        if constexpr (W == 1) {
+          bound = K;
+        } else {
+          if (lane == 0) __hip_atomic_store(tw + w, K, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (b == 0) __syncthreads();  // every wave has a first batch (it may be empty)
+          bound = 0xffffffffu;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const uint32_t o = __hip_atomic_load(tw + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            bound = o < bound ? o : bound;
+          }
+        }
+        thr = fmaxf(thr, below(bound));  // fmaxf takes the other of a NaN
+      }
+      const bool nan = a.s != a.s;  // a NaN or +inf was seen: the vector maxima do not tell
+      int u0 = 0;
+      for (;;) {
+        int stop = U;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u < u0 || u >= stop) continue;
+          if (__ballot(valid[u] && (nan || !(vm[u] <= thr))) == 0) continue;
+          uint64_t mask[N];
+          int total = 0;
+          const int id0 = is_tail ? lo + nv * N + lane : lo + (v0 + u * W * 64) * N;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            mask[i] = __ballot(valid[u] && !(x[u][i] <= thr) && (!is_tail || i == 0));
+            total += __popcll(mask[i]);
+          }
+          if (cnt + total > TOP_CAP) {
+            stop = u;
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (mask[i] == 0) continue;
+            if ((mask[i] >> lane) & 1)
+              cand[cnt + __popcll(mask[i] & ((uint64_t(1) << lane) - 1))] = top_key(x[u][i], id0 + i);
+            cnt += __popcll(mask[i]);
+          }
+        }
+        if (stop == U) break;
+        u0 = stop;
+        top_prune(cand, cnt, k, lane);  // cnt > TOP_CAP - 512 >= k
+        cnt = k;
+        thr = fmaxf(thr, key_value(cand[k - 1]));
+      }
+    }
+  }
+  n_cand = cnt;
+  return a;
+}
+
+// The k largest of a group's candidates into out[0 .. k) as keys, descending (0 after the
+// last one if there are fewer): waves with more than 64 prune, candidates under the
+// last shared bound drop, the rest is ranked by counting.
+template <int W, typename F>
+__device__ __forceinline__ void top_finish(uint64_t* cand, int cnt, const uint32_t* tw, uint32_t bound, uint64_t* merged,
+                                           int* cw, int k, int w, int lane, F emit) {
+  if (cnt > 64) {
+    top_prune(cand, cnt, k, lane);
+    cnt = k;
+  }
+  group_sync<W>();  // every wave's last bound is there
+  if constexpr (W > 1) {
+    bound = tw[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) bound = tw[i] < bound ? tw[i] : bound;
+  }
+  if (bound <= 0x00800000u) bound = 0;
+  const uint64_t mine = lane < cnt ? cand[lane] : 0;
+  const bool in = lane < cnt && static_cast<uint32_t>(mine >> 32) >= bound;
+  const uint64_t mask = __ballot(in);
+  if constexpr (W > 1) {
+    if (lane == 0) cw[w] = __popcll(mask);
+    __syncthreads();
+  }
+  int base = 0, all = W == 1 ? __popcll(mask) : 0;
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      base += i < w ? cw[i] : 0;
+      all += cw[i];
+    }
+  }
+  if (in) merged[base + __popcll(mask & ((uint64_t(1) << lane) - 1))] = mine;
+  group_sync<W>();
+  const int at = w * 64 + lane;
+  if (at < all) {
+    const uint64_t key = merged[at];
+    int rank = 0;
+    for (int i = 0; i < all; ++i) rank += merged[i] > key;
+    if (rank < k) emit(rank, key);
+  }
+  for (int j = all + at; j < k; j += W * 64) emit(j, uint64_t(0));
+}
+
 template <typename F>
 __device__ __forceinline__ float block_reduce(float v, float* red, F f) {
   __syncthreads();
@@ -83,66 +420,189 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // H = log s - sum e^(z - m) (z - m) / s.  A value of -inf has probability 0 and
 // adds nothing; a row without a finite maximum has no distribution (NaN).
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_score(Rows rows, int V, Ids targets, int64_t ignore, int top_k,
-                                                       float* __restrict__ logprob, float* __restrict__ entropy,
-                                                       float2* __restrict__ stats, float* __restrict__ top_lp,
-                                                       int64_t* __restrict__ top_id) {
-  __shared__ float red[TOK_THREADS];
-  __shared__ uint64_t kred[TOK_THREADS];
-  const int64_t r = blockIdx.x;
+struct ScoreOut {
+  float *logprob, *entropy;
+  float2* stats;
+  float* top_lp;
+  int64_t* top_id;
+  int top_k;
+};
+__device__ __forceinline__ void score_padding(const ScoreOut& o, int64_t r, int at, int step) {
+  if (at == 0) {
+    o.logprob[r] = 0.f;
+    if (o.entropy) o.entropy[r] = 0.f;
+    if (o.stats) o.stats[r] = make_float2(0.f, 0.f);
+  }
+  for (int j = at; j < o.top_k; j += step) {
+    o.top_lp[r * o.top_k + j] = 0.f;
+    o.top_id[r * o.top_k + j] = -1;
+  }
+}
+// zy: the target's logit, NaN for a target outside the vocabulary
+__device__ __forceinline__ void score_write(const ScoreOut& o, int64_t r, float m, float s, float t, float zy) {
+  const float ls = logf(s);
+  if (o.logprob) o.logprob[r] = (zy - m) - ls;
+  if (o.entropy) o.entropy[r] = ls - t / s;
+  if (o.stats) o.stats[r] = make_float2(m, ls);
+}
+__device__ __forceinline__ void score_top(const ScoreOut& o, int64_t r, int j, uint64_t key, float m, float ls) {
+  o.top_id[r * o.top_k + j] = 0xffffffffu - static_cast<uint32_t>(key);
+  o.top_lp[r * o.top_k + j] = (key_value(key) - m) - ls;
+}
+
+// Groups of W waves take a row, or one of `parts` ranges of `part_len` values of it
+// (part_sums != NULL: what they found goes there for k_score_join).
+template <typename T, int N, int U, int W, bool TOP>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, int64_t n_rows, int V, Ids targets,
+                                                                 int64_t ignore, ScoreOut out, int parts, int part_len,
+                                                                 float4* __restrict__ part_sums,
+                                                                 uint64_t* __restrict__ part_keys) {
+  constexpr int G = W == 1 ? 4 : 1, WAVES = G * W;
+  __shared__ float slots[W == 1 ? 1 : 3 * W];
+  __shared__ uint64_t cand[TOP ? WAVES * TOP_CAP : 1], merged[TOP ? WAVES * 64 : 1];
+  __shared__ uint32_t tw[WAVES];
+  __shared__ int cw[WAVES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  const int64_t r = part_sums ? item / parts : item;
+  if (r >= n_rows) return;
   const int64_t y = targets.p ? ld_id(targets, r) : 0;
   if (targets.p && y == ignore) {  // padding: nothing of the row is read
-    if (threadIdx.x == 0) {
-      logprob[r] = 0.f;
-      if (entropy) entropy[r] = 0.f;
-      if (stats) stats[r] = make_float2(0.f, 0.f);
-    }
-    for (int j = threadIdx.x; j < top_k; j += TOK_THREADS) {
-      top_lp[r * top_k + j] = 0.f;
-      top_id[r * top_k + j] = -1;
-    }
+    if (!part_sums) score_padding(out, r, w * 64 + lane, W * 64);
     return;
   }
   const T* z = row_ptr<T>(rows, r);
-  float m = -FLT_MAX;
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) m = fmaxf(m, to_f(z[v]));
-  m = block_max(m, red);
-  float s = 0.f, t = 0.f;
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) {
-    const float d = to_f(z[v]) - m, e = exp_f(d);
-    s += e;
-    t += e * fmaxf(d, -1e4f);
+  int lo = 0, hi = V;
+  if (part_sums) {
+    lo = static_cast<int>(item % parts) * part_len;
+    hi = lo + part_len < V ? lo + part_len : V;
   }
-  s = block_sum(s, red);
-  t = block_sum(t, red);
-  const float ls = logf(s);
-  if (threadIdx.x == 0) {
-    if (logprob) logprob[r] = y >= 0 && y < V ? (to_f(z[y]) - m) - ls : __builtin_nanf("");
-    if (entropy) entropy[r] = ls - t / s;
-    if (stats) stats[r] = make_float2(m, ls);
+  float zy = __builtin_nanf("");
+  if (!part_sums && y >= 0 && y < V) zy = to_f(z[y]);
+  uint64_t* mine = cand + (TOP ? wave * TOP_CAP : 0);
+  int cnt = 0;
+  uint32_t bound = 0;
+  Sums a = scan_row<T, N, U, W, SECOND_ENT, TOP>(z, lo, hi, LOG2E, LOG2E, w, lane, out.top_k, mine, tw, cnt, bound);
+  a = group_join<SECOND_ENT, W>(a, slots, w, LOG2E, LOG2E);
+  if (part_sums) {
+    if (w == 0 && lane == 0) part_sums[item] = make_float4(a.m, a.s, a.t, 0.f);
+  } else if (w == 0 && lane == 0) {
+    score_write(out, r, a.m, a.s, a.t, zy);
   }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < top_k; ++j) {
+  if constexpr (TOP) {
+    const float ls = logf(a.s);
+    top_finish<W>(mine, cnt, tw, bound, merged + (W == 1 ? wave * 64 : 0), cw, out.top_k, w, lane,
+                  [&](int j, uint64_t key) {
+                    if (part_sums) part_keys[item * out.top_k + j] = key;
+                    else score_top(out, r, j, key, a.m, ls);
+                  });
+  }
+}
+
+// One block per row joins at most 64 parts: lane p of every wave holds part p's sums; an
+// alternative is at or above K, the ceil(k / q)-th largest of the parts' q-th entries,
+// q = ceil(k / parts).
+constexpr int MAX_PARTS = 64;
+template <typename T>
+__global__ __launch_bounds__(256) void k_score_join(Rows rows, int V, Ids targets, int64_t ignore, ScoreOut out,
+                                                    int parts, const float4* __restrict__ part_sums,
+                                                    const uint64_t* __restrict__ part_keys) {
+  __shared__ uint64_t list[MAX_PARTS * GHM_TOP_MAX];
+  __shared__ int n_list;
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t y = targets.p ? ld_id(targets, r) : 0;
+  if (targets.p && y == ignore) {
+    score_padding(out, r, threadIdx.x, 256);
+    return;
+  }
+  if (threadIdx.x == 0) n_list = 0;
+  Sums a;
+  if (lane < parts) {
+    const float4 v = part_sums[r * parts + lane];
+    a.m = v.x, a.s = v.y, a.t = v.z;
+  }
+  rebase<SECOND_ENT>(a, wave_max(a.m), LOG2E, LOG2E);
+  a.s = wave_sum(a.s);
+  a.t = wave_sum(a.t);
+  if (threadIdx.x == 0)
+    score_write(out, r, a.m, a.s, a.t, y >= 0 && y < V ? to_f(row_ptr<T>(rows, r)[y]) : __builtin_nanf(""));
+  const int k = out.top_k;
+  if (k == 0) return;
+  const float ls = logf(a.s);
+  const uint64_t* keys = part_keys + r * parts * k;
+  const int q = (k + parts - 1) / parts;
+  const uint32_t K = kth_bits(lane < parts ? static_cast<uint32_t>(keys[lane * k + q - 1] >> 32) : 0, (k + q - 1) / q);
+  __syncthreads();
+  for (int i = threadIdx.x; i < parts * k; i += 256) {
+    const uint64_t key = keys[i];
+    if (key != 0 && static_cast<uint32_t>(key >> 32) >= K) list[atomicAdd(&n_list, 1)] = key;
+  }
+  __syncthreads();
+  const int n = n_list;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const uint64_t key = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < k) score_top(out, r, rank, key, a.m, ls);
+  }
+}
+
+// Rows of at most SHORT_V values: one lane per row, the row in registers, the
+// alternatives by k searches.
+constexpr int SHORT_V = 32;
+template <typename T, int M>
+__global__ __launch_bounds__(256) void k_score_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
+                                                     ScoreOut out) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (r >= n_rows) return;
+  const int64_t y = targets.p ? ld_id(targets, r) : 0;
+  if (targets.p && y == ignore) {
+    score_padding(out, r, 0, 1);
+    return;
+  }
+  const T* z = row_ptr<T>(rows, r);
+  float x[M];
+  Sums a;
+#pragma unroll
+  for (int v = 0; v < M; ++v) {
+    x[v] = v < V ? to_f(z[v]) : NEG_INF;
+    a.m = fmaxf(a.m, x[v]);
+  }
+  fold<SECOND_ENT>(a, x, LOG2E, LOG2E);
+  float zy = __builtin_nanf("");
+#pragma unroll
+  for (int v = 0; v < M; ++v)
+    if (v == y && v < V) zy = x[v];
+  score_write(out, r, a.m, a.s, a.t, zy);
+  const float ls = logf(a.s);
+  uint32_t left = V < 32 ? (1u << V) - 1 : 0xffffffffu;
+  for (int j = 0; j < out.top_k; ++j) {
     uint64_t best = 0;
-    for (int v = threadIdx.x; v < V; v += TOK_THREADS) {
-      const uint64_t k = top_key(to_f(z[v]), v);
-      if (k < last && k > best) best = k;
+#pragma unroll
+    for (int v = 0; v < M; ++v) {
+      const uint64_t key = top_key(x[v], v);
+      if (((left >> v) & 1) && key > best) best = key;
     }
-    __syncthreads();
-    kred[threadIdx.x] = best;
-    __syncthreads();
-    for (int w = TOK_THREADS / 2; w >= 1; w >>= 1) {
-      if (threadIdx.x < w && kred[threadIdx.x + w] > kred[threadIdx.x]) kred[threadIdx.x] = kred[threadIdx.x + w];
-      __syncthreads();
-    }
-    last = kred[0];
-    if (threadIdx.x == 0) {
-      const uint32_t v = 0xffffffffu - static_cast<uint32_t>(last);
-      top_id[r * top_k + j] = v;
-      top_lp[r * top_k + j] = (to_f(z[v]) - m) - ls;
-    }
+    left &= ~(1u << (0xffffffffu - static_cast<uint32_t>(best)));
+    score_top(out, r, j, best, a.m, ls);
   }
+}
+
+// How a row is split (both kinds of logits operator): rows few and long go in parts so
+// that about 512 groups are at work, each with at least one vector per lane of 8 waves.
+struct Split {
+  int parts, len;
+};
+inline Split row_split(int64_t rows, int64_t V) {
+  const int64_t most = V / 4096;
+  int64_t p = rows > 0 && rows < 512 ? (512 + rows - 1) / rows : 1;
+  if (p > most) p = most;
+  if (p > MAX_PARTS) p = MAX_PARTS;
+  if (p < 2) return {1, static_cast<int>(V)};
+  int64_t len = (V + p - 1) / p;
+  len = (len + 511) / 512 * 512;
+  return {static_cast<int>((V + len - 1) / len), static_cast<int>(len)};
 }
 
 // dz_v = -p_v [g_lp + sum_j g_top_j + g_H (log p_v + H)] + g_lp [v = y] + sum_j g_top_j [v = id_j]
@@ -379,9 +839,46 @@ inline bool dtype_ok(int d) { return d >= 0 && d <= 2; }
   GHM_CHECK(n_inner >= 1 && s_outer >= 0 && s_inner >= 0, "row strides")
 
 extern "C" int64_t ghm_token_logprobs_ws(int64_t rows, int64_t V, int top_k, int dtype) {
-  (void)rows; (void)V; (void)top_k; (void)dtype;
-  return 0;
+  (void)dtype;
+  if (rows <= 0 || V <= 0 || top_k < 0) return 0;
+  const Split p = row_split(rows, V);
+  return p.parts == 1 ? 0 : rows * p.parts * (16 + 8 * static_cast<int64_t>(top_k));
 }
+
+namespace {
+template <typename T, int N, int U, int W>
+void launch_score(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreOut& o, const Split& p,
+                  void* ws, hipStream_t s) {
+  constexpr int G = W == 1 ? 4 : 1;
+  float4* sums = p.parts > 1 ? static_cast<float4*>(ws) : nullptr;
+  uint64_t* keys = sums ? reinterpret_cast<uint64_t*>(sums + rows * p.parts) : nullptr;
+  const dim3 g(static_cast<unsigned>((rows * p.parts + G - 1) / G)), b(64 * G * W);
+  if (o.top_k)
+    hipLaunchKernelGGL((k_score<T, N, U, W, true>), g, b, 0, s, m, rows, V, t, ignore, o, p.parts, p.len, sums, keys);
+  else
+    hipLaunchKernelGGL((k_score<T, N, U, W, false>), g, b, 0, s, m, rows, V, t, ignore, o, p.parts, p.len, sums, keys);
+  if (sums)
+    hipLaunchKernelGGL(k_score_join<T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, m, V, t, ignore, o, p.parts,
+                       sums, keys);
+}
+template <typename T>
+void score_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreOut& o, void* ws,
+               hipStream_t s) {
+  const Split p = row_split(rows, V);
+  constexpr int N = Vec<T>::N;
+  if (V <= SHORT_V) {
+    const dim3 g(static_cast<unsigned>((rows + 255) / 256));
+    if (V <= 12) hipLaunchKernelGGL((k_score_short<T, 12>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
+    else hipLaunchKernelGGL((k_score_short<T, SHORT_V>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
+  } else if (V <= 512) {
+    launch_score<T, 1, 8, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (V <= 2048) {
+    launch_score<T, N, 4, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else {
+    launch_score<T, N, 4, 8>(m, rows, V, t, ignore, o, p, ws, s);
+  }
+}
+}  // namespace
 
 extern "C" int ghm_token_logprobs(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner,
                                   int64_t rows, int64_t V, const void* targets, int id_bits, int64_t ignore_index,
@@ -392,14 +889,14 @@ extern "C" int ghm_token_logprobs(const void* logits, int dtype, int64_t n_inner
   GHM_CHECK(!targets || ids_ok(id_bits), "id_bits (8, 32, 64)");
   GHM_CHECK(rows == 0 || (logits && (!targets || logprob) && (!logprob || targets) &&
                           (top_k == 0 || (top_logprob && top_id))), "null pointer");
-  GHM_CHECK(ws_bytes >= ghm_token_logprobs_ws(rows, V, top_k, dtype), "workspace too small");
-  (void)ws;
+  const int64_t need = ghm_token_logprobs_ws(rows, V, top_k, dtype);
+  GHM_CHECK(ws_bytes >= need && (need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
+            "workspace (too small, or not 16-byte aligned)");
   if (rows == 0) return GHM_OK;
   const Rows m{logits, n_inner, s_outer, s_inner};
-  const Ids t{targets, id_bits};
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_score<T>, dim3(static_cast<unsigned>(rows)), dim3(TOK_THREADS), 0,
-                                         ghm_stream(stream), m, static_cast<int>(V), t, ignore_index, top_k, logprob,
-                                         entropy, reinterpret_cast<float2*>(stats), top_logprob, top_id));
+  const ScoreOut o{logprob, entropy, reinterpret_cast<float2*>(stats), top_logprob, top_id, top_k};
+  TOK_DISPATCH(dtype, score_any<T>(m, rows, static_cast<int>(V), Ids{targets, id_bits}, ignore_index, o, ws,
+                                   ghm_stream(stream)));
   return ghm_launch_status();
 }
 
