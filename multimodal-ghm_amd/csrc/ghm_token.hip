@@ -199,13 +199,16 @@ __device__ __forceinline__ Sums group_join(Sums a, float* slots, int w, float c1
 }
 
 // ---- the largest values of a row, found in the same pass -------------------
-// Each wave keeps candidates (64-bit keys) in LDS: the values above a threshold that
-// only rises.  Valid thresholds: (a) with r = ceil(k / W), the least over the waves of
-// each wave's r-th largest lane maximum: the waves hold k values at or above it;
-// (b) a wave's own k-th candidate after a prune, strictly, for its later (higher) ids.
-// A few hundred of a row's values become candidates; the k best of them are ranked at
-// the end by counting.
-constexpr int TOP_CAP = 576;  // 64 kept by a prune + one vector of 8 values per lane
+// The unit kept is a lane's vector of N values, by its maximum (value descending, index
+// ascending, as a 64-bit key): the k largest values lie in the k largest vectors, since
+// each of k vectors ranked above another holds a value that ranks above all of that one's.
+// A wave notes in LDS the vectors above a threshold that only rises.  Valid thresholds:
+// (a) with r = ceil(k / W), the least over the waves of each wave's r-th largest lane
+// maximum: the waves hold k vectors at or above it; (b) a wave's own k-th vector after a
+// prune, strictly, for its later (higher) indices.  That is one comparison per vector, and
+// a few hundred vectors of a row are noted; at the end they are ranked by counting, and
+// the values of the k best ones, read again, are ranked the same way.
+constexpr int TOP_CAP = 256;  // vectors noted per wave: 64 kept by a prune, 64 per step
 
 // at least r lanes hold u >= the result (its upper 16 bits are searched: a lower bound
 // of the r-th largest); 0: fewer
@@ -253,36 +256,44 @@ __device__ __forceinline__ void top_prune(uint64_t* cand, int n, int k, int lane
   wave_fence();
 }
 
-// A row's values lo .. hi - 1, lane by lane: batches of U vectors of N values; the
-// values after the last whole vector go to wave 0.  Vectors and batches of a wave come
-// in ascending order.  TOP: k candidates are kept in cand (n of them on return), thr
-// and the shared lane-maximum bounds tw as above.
+// What finding the alternatives takes in LDS per group of W waves.
+template <int N, int W>
+struct TopLds {
+  uint64_t cand[W * TOP_CAP], merged[W * 64], best[N == 1 ? 1 : GHM_TOP_MAX], vals[N == 1 ? 1 : GHM_TOP_MAX * N];
+  uint32_t bound[W];
+  int count[W], n_vals;
+};
+struct TopState {
+  int cnt = 0;         // vectors this wave has noted
+  uint32_t bound = 0;  // the group's bound (a) as order bits
+};
+
+// A row's values lo .. hi - 1: batches of U vectors of N values per lane; the values
+// after the last whole vector are one more vector, of lane 0 of wave 0.  The vectors of a
+// wave come in ascending order.  TOP: notes vectors for the k largest values.
 template <typename T, int N, int U, int W, int SECOND, bool TOP>
 __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, float c2, int w, int lane, int k,
-                                         uint64_t* cand, uint32_t* tw, int& n_cand, uint32_t& bound) {
+                                         TopLds<N, W>* lds, TopState& top) {
   Sums a;
   float thr = __builtin_nanf("");
-  int cnt = 0;
   const int nv = (hi - lo) / N, tail = (hi - lo) - nv * N;
   const int r = TOP ? (k + W - 1) / W : 0;
   constexpr int STEP = W * 64 * U;
-  const int nb = (nv + STEP - 1) / STEP + (tail && N > 1 ? 1 : 0);  // the tail is one batch of its own
-  const int full = (nv + STEP - 1) / STEP;
+  const int full = (nv + STEP - 1) / STEP, nb = full + (tail ? 1 : 0);
+  uint64_t* cand = TOP ? lds->cand + w * TOP_CAP : nullptr;
   for (int b = 0; b < nb; ++b) {
     float x[U][N], vm[U];
-    bool valid[U];
-    const bool is_tail = b == full;
-    const int v0 = b * STEP + w * 64 + lane;
+    const int v0 = b < full ? b * STEP + w * 64 + lane : nv + w * 64 + lane;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      valid[u] = !is_tail && v0 + u * W * 64 < nv;
 #pragma unroll
       for (int i = 0; i < N; ++i) x[u][i] = NEG_INF;
-      if (valid[u]) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
+      if (v0 + u * W * 64 < nv) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
     }
-    if (is_tail) {
-      valid[0] = w == 0 && lane < tail;
-      if (valid[0]) x[0][0] = to_f(z[lo + nv * N + lane]);
+    if (N > 1 && b == full && v0 == nv) {
+#pragma unroll
+      for (int i = 0; i < N - 1; ++i)
+        if (i < tail) x[0][i] = to_f(z[lo + nv * N + i]);
     }
     float bm = -FLT_MAX;
 #pragma unroll
@@ -296,105 +307,121 @@ __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, f
 #pragma unroll
     for (int u = 0; u < U; ++u) fold<SECOND>(a, x[u], c1, c2);
     if constexpr (TOP) {
-      // refresh the shared bound after batches 1, 2, 4, 8, ... and the last
-      if (((b + 1) & b) == 0 || b == nb - 1) {
+      if (((b + 1) & b) == 0 || b == nb - 1) {  // the shared bound, after batches 1, 2, 4, 8, ... and the last
         const uint32_t K = kth_bits(order_bits(a.m), r);
-        if constexpr (W == 1) {
-          bound = K;
-        } else {
-          if (lane == 0) __hip_atomic_store(tw + w, K, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          if (b == 0) __syncthreads();  // every wave has a first batch (it may be empty)
-          bound = 0xffffffffu;
+        top.bound = K;
+        if constexpr (W > 1) {
+          if (lane == 0) __hip_atomic_store(lds->bound + w, K, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (b == 0) __syncthreads();
 #pragma unroll
           for (int i = 0; i < W; ++i) {
-            const uint32_t o = __hip_atomic_load(tw + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            bound = o < bound ? o : bound;
+            const uint32_t o = __hip_atomic_load(lds->bound + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            top.bound = o < top.bound ? o : top.bound;
           }
         }
-        thr = fmaxf(thr, below(bound));  // fmaxf takes the other of a NaN
+        thr = fmaxf(thr, below(top.bound));  // fmaxf takes the other of a NaN
       }
-      const bool nan = a.s != a.s;  // a NaN or +inf was seen: the vector maxima do not tell
-      int u0 = 0;
-      for (;;) {
-        int stop = U;
+      const bool nan = a.s != a.s;  // a NaN or +inf was seen; the maxima skip NaN
+      if (__ballot(nan || !(bm <= thr)) == 0) continue;
+      if (__ballot(nan)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (u < u0 || u >= stop) continue;
-          if (__ballot(valid[u] && (nan || !(vm[u] <= thr))) == 0) continue;
-          uint64_t mask[N];
-          int total = 0;
-          const int id0 = is_tail ? lo + nv * N + lane : lo + (v0 + u * W * 64) * N;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            mask[i] = __ballot(valid[u] && !(x[u][i] <= thr) && (!is_tail || i == 0));
-            total += __popcll(mask[i]);
-          }
-          if (cnt + total > TOP_CAP) {
-            stop = u;
-            continue;
-          }
+          for (int i = 0; i < N; ++i) vm[u] = x[u][i] != x[u][i] ? x[u][i] : vm[u];
+      }
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (mask[i] == 0) continue;
-            if ((mask[i] >> lane) & 1)
-              cand[cnt + __popcll(mask[i] & ((uint64_t(1) << lane) - 1))] = top_key(x[u][i], id0 + i);
-            cnt += __popcll(mask[i]);
-          }
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * W * 64;
+        const bool valid = v < nv + (tail && b == full);
+        uint64_t mask = __ballot(valid && !(vm[u] <= thr));
+        if (mask == 0) continue;
+        if (top.cnt + __popcll(mask) > TOP_CAP) {
+          top_prune(cand, top.cnt, k, lane);
+          top.cnt = k;  // of at least TOP_CAP - 63 > k
+          thr = fmaxf(thr, key_value(cand[k - 1]));
+          mask = __ballot(valid && !(vm[u] <= thr));
         }
-        if (stop == U) break;
-        u0 = stop;
-        top_prune(cand, cnt, k, lane);  // cnt > TOP_CAP - 512 >= k
-        cnt = k;
-        thr = fmaxf(thr, key_value(cand[k - 1]));
+        if ((mask >> lane) & 1) cand[top.cnt + __popcll(mask & ((uint64_t(1) << lane) - 1))] = top_key(vm[u], v);
+        top.cnt += __popcll(mask);
       }
     }
   }
-  n_cand = cnt;
   return a;
 }
 
-// The k largest of a group's candidates into out[0 .. k) as keys, descending (0 after the
-// last one if there are fewer): waves with more than 64 prune, candidates under the
-// last shared bound drop, the rest is ranked by counting.
-template <int W, typename F>
-__device__ __forceinline__ void top_finish(uint64_t* cand, int cnt, const uint32_t* tw, uint32_t bound, uint64_t* merged,
-                                           int* cw, int k, int w, int lane, F emit) {
-  if (cnt > 64) {
-    top_prune(cand, cnt, k, lane);
-    cnt = k;
+// emit(rank, key) for the k largest values of the group's range (key 0 past the last one
+// if it holds fewer): the noted vectors at or above the last bound are ranked, then the
+// values of the k best that reach the k-th vector's maximum.
+template <typename T, int N, int W, typename F>
+__device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N, W>* lds, TopState top, int k, int w,
+                                           int lane, F emit) {
+  uint64_t* cand = lds->cand + w * TOP_CAP;
+  if (top.cnt > 64) {
+    top_prune(cand, top.cnt, k, lane);
+    top.cnt = k;
   }
   group_sync<W>();  // every wave's last bound is there
+  uint32_t bound = top.bound;
   if constexpr (W > 1) {
-    bound = tw[0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) bound = tw[i] < bound ? tw[i] : bound;
+    for (int i = 0; i < W; ++i) bound = lds->bound[i] < bound ? lds->bound[i] : bound;
   }
   if (bound <= 0x00800000u) bound = 0;
-  const uint64_t mine = lane < cnt ? cand[lane] : 0;
-  const bool in = lane < cnt && static_cast<uint32_t>(mine >> 32) >= bound;
+  const uint64_t mine = lane < top.cnt ? cand[lane] : 0;
+  const bool in = lane < top.cnt && static_cast<uint32_t>(mine >> 32) >= bound;
   const uint64_t mask = __ballot(in);
+  int base = 0, all = __popcll(mask);
   if constexpr (W > 1) {
-    if (lane == 0) cw[w] = __popcll(mask);
+    if (lane == 0) lds->count[w] = all;
+    if (w == 0 && lane == 0) lds->n_vals = 0;
     __syncthreads();
-  }
-  int base = 0, all = W == 1 ? __popcll(mask) : 0;
-  if constexpr (W > 1) {
+    all = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      base += i < w ? cw[i] : 0;
-      all += cw[i];
+      base += i < w ? lds->count[i] : 0;
+      all += lds->count[i];
     }
+  } else if (lane == 0) {
+    lds->n_vals = 0;
   }
-  if (in) merged[base + __popcll(mask & ((uint64_t(1) << lane) - 1))] = mine;
+  if (in) lds->merged[base + __popcll(mask & ((uint64_t(1) << lane) - 1))] = mine;
   group_sync<W>();
   const int at = w * 64 + lane;
   if (at < all) {
-    const uint64_t key = merged[at];
+    const uint64_t key = lds->merged[at];
     int rank = 0;
-    for (int i = 0; i < all; ++i) rank += merged[i] > key;
-    if (rank < k) emit(rank, key);
+#pragma unroll 4
+    for (int i = 0; i < all; ++i) rank += lds->merged[i] > key;
+    if constexpr (N == 1) {
+      if (rank < k) emit(rank, (key & 0xffffffff00000000ull) | (static_cast<uint32_t>(key) - lo));
+    } else {
+      if (rank < k) lds->best[rank] = key;
+    }
   }
-  for (int j = all + at; j < k; j += W * 64) emit(j, uint64_t(0));
+  if constexpr (N == 1) {
+    for (int j = all + at; j < k; j += W * 64) emit(j, uint64_t(0));
+  } else {
+    group_sync<W>();
+    const int nb = all < k ? all : k;
+    const uint32_t least = all < k ? 0 : static_cast<uint32_t>(lds->best[k - 1] >> 32);
+    for (int i = at; i < nb * N; i += W * 64) {
+      const int id = lo + static_cast<int>(0xffffffffu - static_cast<uint32_t>(lds->best[i / N])) * N + i % N;
+      if (id < hi) {
+        const uint64_t key = top_key(to_f(z[id]), id);
+        if (static_cast<uint32_t>(key >> 32) >= least) lds->vals[atomicAdd(&lds->n_vals, 1)] = key;
+      }
+    }
+    group_sync<W>();
+    const int n = lds->n_vals;
+    for (int i = at; i < n; i += W * 64) {
+      const uint64_t key = lds->vals[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += lds->vals[j] > key;
+      if (rank < k) emit(rank, key);
+    }
+    for (int j = n + at; j < k; j += W * 64) emit(j, uint64_t(0));
+  }
 }
 
 template <typename F>
@@ -457,11 +484,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
                                                                  int64_t ignore, ScoreOut out, int parts, int part_len,
                                                                  float4* __restrict__ part_sums,
                                                                  uint64_t* __restrict__ part_keys) {
-  constexpr int G = W == 1 ? 4 : 1, WAVES = G * W;
+  constexpr int G = W == 1 ? 4 : 1;
   __shared__ float slots[W == 1 ? 1 : 3 * W];
-  __shared__ uint64_t cand[TOP ? WAVES * TOP_CAP : 1], merged[TOP ? WAVES * 64 : 1];
-  __shared__ uint32_t tw[WAVES];
-  __shared__ int cw[WAVES];
+  __shared__ TopLds<N, TOP ? W : 1> top_lds[TOP ? G : 1];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W;
   const int64_t r = part_sums ? item / parts : item;
@@ -479,10 +504,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
   }
   float zy = __builtin_nanf("");
   if (!part_sums && y >= 0 && y < V) zy = to_f(z[y]);
-  uint64_t* mine = cand + (TOP ? wave * TOP_CAP : 0);
-  int cnt = 0;
-  uint32_t bound = 0;
-  Sums a = scan_row<T, N, U, W, SECOND_ENT, TOP>(z, lo, hi, LOG2E, LOG2E, w, lane, out.top_k, mine, tw, cnt, bound);
+  TopLds<N, W>* lds = nullptr;
+  if constexpr (TOP) lds = top_lds + wave / W;
+  TopState top;
+  Sums a = scan_row<T, N, U, W, SECOND_ENT, TOP>(z, lo, hi, LOG2E, LOG2E, w, lane, out.top_k, lds, top);
   a = group_join<SECOND_ENT, W>(a, slots, w, LOG2E, LOG2E);
   if (part_sums) {
     if (w == 0 && lane == 0) part_sums[item] = make_float4(a.m, a.s, a.t, 0.f);
@@ -491,11 +516,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
   }
   if constexpr (TOP) {
     const float ls = logf(a.s);
-    top_finish<W>(mine, cnt, tw, bound, merged + (W == 1 ? wave * 64 : 0), cw, out.top_k, w, lane,
-                  [&](int j, uint64_t key) {
-                    if (part_sums) part_keys[item * out.top_k + j] = key;
-                    else score_top(out, r, j, key, a.m, ls);
-                  });
+    top_finish<T>(z, lo, hi, lds, top, out.top_k, w, lane, [&](int j, uint64_t key) {
+      if (part_sums) part_keys[item * out.top_k + j] = key;
+      else score_top(out, r, j, key, a.m, ls);
+    });
   }
 }
 
