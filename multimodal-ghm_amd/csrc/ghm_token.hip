@@ -26,9 +26,6 @@ __device__ __forceinline__ void from_f(float& o, float x) { o = x; }
 __device__ __forceinline__ void from_f(bf16_t& o, float x) { o.u = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
 __device__ __forceinline__ void from_f(f16_t& o, float x) { o.h = static_cast<_Float16>(x); }
 
-// e^x from the exponent's own 32-bit unit: 2^(x log2 e), 0 below the f32 range
-__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
-
 struct Rows {
   const void* base;
   int64_t n_inner, s_outer, s_inner;
@@ -424,24 +421,6 @@ __device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N,
   }
 }
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float* red, F f) {
-  __syncthreads();
-  red[threadIdx.x] = v;
-  __syncthreads();
-  for (int s = TOK_THREADS / 2; s >= 1; s >>= 1) {
-    if (threadIdx.x < s) red[threadIdx.x] = f(red[threadIdx.x], red[threadIdx.x + s]);
-    __syncthreads();
-  }
-  return red[0];
-}
-__device__ __forceinline__ float block_max(float v, float* red) {
-  return block_reduce(v, red, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  return block_reduce(v, red, [](float a, float b) { return a + b; });
-}
-
 // ---------------------------------------------------------------------------
 // Scores: m = max z, s = sum e^(z - m), log p_v = (z_v - m) - log s,
 // H = log s - sum e^(z - m) (z - m) / s.  A value of -inf has probability 0 and
@@ -629,37 +608,138 @@ inline Split row_split(int64_t rows, int64_t V) {
   return {static_cast<int>((V + len - 1) / len), static_cast<int>(len)};
 }
 
+// f(value, index) over a row's values lo .. hi - 1, written to d: batches of U vectors
+template <typename T, int N, int U, int W, typename F>
+__device__ __forceinline__ void map_row(const T* z, T* d, int lo, int hi, int w, int lane, F f) {
+  const int nv = (hi - lo) / N;
+  constexpr int STEP = W * 64 * U;
+  for (int v0 = w * 64 + lane; v0 < nv; v0 += STEP) {
+    float x[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * W * 64 < nv) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * W * 64 >= nv) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = f(x[u][i]);
+      store_vec<N>(d + lo + (v0 + u * W * 64) * N, x[u]);
+    }
+  }
+  if constexpr (N > 1) {
+    const int v = lo + nv * N + w * 64 + lane;
+    if (v < hi) from_f(d[v], f(to_f(z[v])));
+  }
+}
+template <typename T, int N, int W>
+__device__ __forceinline__ void zero_row(T* d, int lo, int hi, int w, int lane) {
+  const int nv = (hi - lo) / N;
+  float x[N] = {};
+  for (int v = w * 64 + lane; v < nv; v += W * 64) store_vec<N>(d + lo + v * N, x);
+  if constexpr (N > 1) {
+    const int v = lo + nv * N + w * 64 + lane;
+    if (v < hi) from_f(d[v], 0.f);
+  }
+}
+
 // dz_v = -p_v [g_lp + sum_j g_top_j + g_H (log p_v + H)] + g_lp [v = y] + sum_j g_top_j [v = id_j]
-template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_score_bwd(Rows rows, int V, Ids targets, int64_t ignore, int top_k,
-                                                           const int64_t* __restrict__ top_id,
-                                                           const float2* __restrict__ stats,
-                                                           const float* __restrict__ entropy,
-                                                           const float* __restrict__ g_lp,
-                                                           const float* __restrict__ g_ent,
-                                                           const float* __restrict__ g_top, T* __restrict__ dz) {
-  const int64_t r = blockIdx.x;
+struct ScoreGrad {
+  const int64_t* top_id;
+  const float2* stats;
+  const float *entropy, *g_lp, *g_ent, *g_top;
+  int top_k;
+};
+struct ScoreRow {  // the gradient at a value z other than the target and the alternatives
+  float m, c, gs, g2, gh;
+  __device__ __forceinline__ float operator()(float z) const {
+    const float d = z - m;
+    return -__builtin_amdgcn_exp2f(__builtin_fmaf(d, LOG2E, c)) * __builtin_fmaf(g2, fmaxf(d, -1e4f), gh);
+  }
+};
+__device__ __forceinline__ ScoreRow score_row(const ScoreGrad& g, int64_t r, float g1, float top_sum) {
+  ScoreRow o;
+  const float2 st = g.stats[r];
+  o.m = st.x;
+  o.c = -st.y * LOG2E;
+  o.gs = g1 + top_sum;
+  o.g2 = g.g_ent ? g.g_ent[r] : 0.f;
+  o.gh = g.g_ent ? __builtin_fmaf(o.g2, g.entropy[r] - st.y, o.gs) : o.gs;
+  return o;
+}
+
+// the whole row part is written first, then the target's and the alternatives' entries again
+template <typename T, int N, int U, int W>
+__global__ __launch_bounds__(256) void k_score_bwd(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
+                                                   ScoreGrad g, int parts, int part_len, T* __restrict__ dz) {
+  constexpr int G = 4 / W;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W, r = item / parts;
+  if (r >= n_rows) return;
+  const int lo = static_cast<int>(item % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
   T* d = dz + r * V;
-  const int64_t y = targets.p ? ld_id(targets, r) : 0;
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
   if (targets.p && y == ignore) {
-    for (int v = threadIdx.x; v < V; v += TOK_THREADS) from_f(d[v], 0.f);
+    zero_row<T, N, W>(d, lo, hi, w, lane);
     return;
   }
   const T* z = row_ptr<T>(rows, r);
-  const float2 st = stats[r];
-  float g1 = g_lp ? g_lp[r] : 0.f;
-  if (g_lp && (y < 0 || y >= V)) g1 = __builtin_nanf("");
-  const float g2 = g_ent ? g_ent[r] : 0.f, H = g_ent ? entropy[r] : 0.f;
-  float gs = g1;
-  for (int j = 0; j < top_k; ++j) gs += g_top[r * top_k + j];
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) {
-    const float lp = (to_f(z[v]) - st.x) - st.y, p = exp_f(lp);
-    float g = -p * (gs + g2 * (fmaxf(lp, -1e4f) + H));
-    if (g_lp && v == y) g += g1;
-    for (int j = 0; j < top_k; ++j)
-      if (top_id[r * top_k + j] == v) g += g_top[r * top_k + j];
-    from_f(d[v], g);
+  float g1 = g.g_lp ? g.g_lp[r] : 0.f;
+  if (g.g_lp && (y < 0 || y >= V)) g1 = __builtin_nanf("");
+  float top = 0.f;
+  if (g.g_top) top = wave_sum(lane < g.top_k ? g.g_top[r * g.top_k + lane] : 0.f);
+  const ScoreRow f = score_row(g, r, g1, top);
+  map_row<T, N, U, W>(z, d, lo, hi, w, lane, f);
+  group_sync<W>();
+  if (w != 0) return;
+  const int64_t id = g.g_top && lane < g.top_k ? g.top_id[r * g.top_k + lane] : -1;
+  if (id >= lo && id < hi)
+    from_f(d[id], f(to_f(z[id])) + g.g_top[r * g.top_k + lane] + (g.g_lp && id == y ? g1 : 0.f));
+  if (g.g_lp && y >= lo && y < hi && __ballot(id == y) == 0 && lane == 0) from_f(d[y], f(to_f(z[y])) + g1);
+}
+
+template <typename T, int M>
+__global__ __launch_bounds__(256) void k_score_bwd_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
+                                                         ScoreGrad g, T* __restrict__ dz) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (r >= n_rows) return;
+  T* d = dz + r * V;
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  if (targets.p && y == ignore) {
+    for (int v = 0; v < V; ++v) from_f(d[v], 0.f);
+    return;
   }
+  const T* z = row_ptr<T>(rows, r);
+  float x[M], own[M];
+#pragma unroll
+  for (int v = 0; v < M; ++v) {
+    x[v] = v < V ? to_f(z[v]) : 0.f;
+    own[v] = 0.f;
+  }
+  float g1 = g.g_lp ? g.g_lp[r] : 0.f, top = 0.f;
+  if (g.g_lp && (y < 0 || y >= V)) g1 = __builtin_nanf("");
+  if (g.g_top)
+    for (int j = 0; j < g.top_k; ++j) {
+      const float t = g.g_top[r * g.top_k + j];
+      const int64_t id = g.top_id[r * g.top_k + j];
+      top += t;
+#pragma unroll
+      for (int v = 0; v < M; ++v) own[v] += v == id ? t : 0.f;
+    }
+  const ScoreRow f = score_row(g, r, g1, top);
+#pragma unroll
+  for (int v = 0; v < M; ++v)
+    if (v < V) from_f(d[v], f(x[v]) + own[v] + (g.g_lp && v == y ? g1 : 0.f));
+}
+
+// How the elementwise passes split rows over groups of 4 waves: at least 2048 groups
+// where the rows are long enough, of at least 4096 values each.
+inline Split map_split(int64_t rows, int64_t V) {
+  int64_t p = rows > 0 && rows < 2048 ? (2048 + rows - 1) / rows : 1;
+  if (p > V / 4096) p = V / 4096;
+  if (p < 2) return {1, static_cast<int>(V)};
+  int64_t len = (V + p - 1) / p;
+  len = (len + 511) / 512 * 512;
+  return {static_cast<int>((V + len - 1) / len), static_cast<int>(len)};
 }
 
 // ---------------------------------------------------------------------------
@@ -681,143 +761,408 @@ __device__ __forceinline__ float ld_teacher(const Teacher& t, int64_t i) {
 __device__ __forceinline__ bool teacher_has(const Teacher& t, int64_t i) {
   return ld_id(t.ids, i) >= 0 && !(ld_teacher(t, i) == NEG_INF);
 }
-// rows that count: the target is not the ignored one; without targets, an alternative is present
-__device__ __forceinline__ bool row_counts(const Teacher& t, const Ids& targets, int64_t ignore, int64_t r) {
+// rows that count: the target is not the ignored one; without targets, an alternative is
+// present.  Asked by the whole group, answered alike in every lane.
+__device__ __forceinline__ bool row_counts(const Teacher& t, const Ids& targets, int64_t ignore, int64_t r, int lane) {
   if (targets.p) return ld_id(targets, r) != ignore;
-  for (int j = 0; j < t.k; ++j)
-    if (teacher_has(t, r * t.k + j)) return true;
+  for (int j = lane; j - lane < t.k; j += 64)
+    if (__ballot(j < t.k && teacher_has(t, r * t.k + j))) return true;
   return false;
 }
 
-// norm[0] = 1 / max(number of counted rows, 1)
-__global__ __launch_bounds__(TOK_THREADS) void k_distill_count(Teacher t, Ids targets, int64_t ignore, int64_t n,
-                                                               float* __restrict__ norm) {
-  __shared__ int red[TOK_THREADS];
-  int c = 0;
-  for (int64_t r = threadIdx.x; r < n; r += TOK_THREADS) c += row_counts(t, targets, ignore, r);
-  red[threadIdx.x] = c;
-  __syncthreads();
-  for (int s = TOK_THREADS / 2; s >= 1; s >>= 1) {
-    if (threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
-    __syncthreads();
+struct Mix {  // c1: exponent factor of the row's first sum (log2 e, or log2 e / tau); c2 of the second
+  float tau, it, alpha, c1, c2;
+  bool hard, two;  // two: the hard labels' softmax and the teacher's are different ones
+};
+// what scales the gradient: grad_scale * upstream / counted rows
+struct Upstream {
+  const int* counts;  // counted rows per block of k_distill_count
+  int n_counts;
+  const float* norm;
+  const float* up;
+  int up_rows;
+  float scale;
+};
+__device__ __forceinline__ float upstream(const Upstream& u, int64_t r, int lane) {
+  float s = u.scale;
+  if (u.counts) {
+    int c = lane < u.n_counts ? u.counts[lane] : 0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o, 64);
+    s *= 1.f / static_cast<float>(c > 1 ? c : 1);
   }
-  if (threadIdx.x == 0) norm[0] = 1.f / static_cast<float>(red[0] > 1 ? red[0] : 1);
+  if (u.norm) s *= u.norm[0];
+  if (u.up) s *= u.up[u.up_rows ? r : 0];
+  return s;
 }
 
-// row_stats: (m, log s at 1, log s at tau, unused)
-template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_distill_rows(Rows rows, int V, Teacher tc, Ids targets,
-                                                              int64_t ignore, float tau, float alpha,
-                                                              float* __restrict__ row_loss,
-                                                              float4* __restrict__ row_stats) {
-  __shared__ float red[TOK_THREADS];
+constexpr int MAX_COUNTS = 64;
+__global__ __launch_bounds__(256) void k_distill_count(Teacher t, Ids targets, int64_t ignore, int64_t n, int64_t per,
+                                                       int* __restrict__ counts) {
+  __shared__ int red[4];
+  const int64_t lo = blockIdx.x * per, hi = lo + per < n ? lo + per : n;
+  int c = 0;
+  for (int64_t r = lo + threadIdx.x; r < hi; r += 256) {
+    bool in = false;
+    if (targets.p) {
+      in = ld_id(targets, r) != ignore;
+    } else {
+      for (int j = 0; j < t.k && !in; ++j) in = teacher_has(t, r * t.k + j);
+    }
+    c += in;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// the sum of row losses and the number of counted rows of one range of rows, in a fixed
+// order; a single block (or the second stage, over the ranges' results) writes the loss
+__device__ __forceinline__ void distill_result(float s, int c, int mean, float* loss, float* norm) {
+  const float inv = 1.f / static_cast<float>(c > 1 ? c : 1);
+  if (mean) norm[0] = inv;
+  loss[0] = mean ? s * inv : s;
+}
+__global__ __launch_bounds__(1024) void k_distill_total(const float* __restrict__ row_loss,
+                                                        const float4* __restrict__ row_stats, int64_t n, int64_t per,
+                                                        float2* __restrict__ parts, int mean,
+                                                        float* __restrict__ loss, float* __restrict__ norm) {
+  __shared__ float rs[16];
+  __shared__ int rc[16];
+  const int64_t lo = blockIdx.x * per, hi = lo + per < n ? lo + per : n;
+  float s = 0.f;
+  int c = 0;
+#pragma unroll 8
+  for (int64_t r = lo + threadIdx.x; r < hi; r += 1024) {
+    s += row_loss[r];
+    c += row_stats[r].w != 0.f;
+  }
+  s = wave_sum(s);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o, 64);
+  if ((threadIdx.x & 63) == 0) {
+    rs[threadIdx.x >> 6] = s;
+    rc[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = 0.f, c = 0;
+  for (int i = 0; i < 16; ++i) {
+    s += rs[i];
+    c += rc[i];
+  }
+  if (gridDim.x == 1) distill_result(s, c, mean, loss, norm);
+  else parts[blockIdx.x] = make_float2(s, __int_as_float(c));
+}
+__global__ __launch_bounds__(64) void k_distill_total2(const float2* __restrict__ parts, int n, int mean,
+                                                       float* __restrict__ loss, float* __restrict__ norm) {
+  const float2 v = static_cast<int>(threadIdx.x) < n ? parts[threadIdx.x] : make_float2(0.f, 0.f);
+  const float s = wave_sum(v.x);
+  int c = __float_as_int(v.y);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o, 64);
+  if (threadIdx.x == 0) distill_result(s, c, mean, loss, norm);
+}
+
+// A row's teacher in LDS: ids (-1 absent) and q; log q = (t - mt) it - lt.
+template <int W>
+struct TeacherLds {
+  int id[GHM_DISTILL_MAX];
+  float q[GHM_DISTILL_MAX], slots[8 * W];
+};
+struct TeacherRow {
+  float mt, lt;
+  bool some, bad;  // an entry is present; one lies outside the vocabulary
+};
+template <int W>
+__device__ __forceinline__ TeacherRow teacher_row(const Teacher& t, int64_t r, int V, float it, TeacherLds<W>& lds,
+                                                  int w, int lane) {
+  TeacherRow o;
+  float mt = -FLT_MAX, bad = 0.f;
+  for (int j = w * 64 + lane; j < t.k; j += W * 64) {
+    const int64_t id = ld_id(t.ids, r * t.k + j);
+    const float x = ld_teacher(t, r * t.k + j);
+    const bool has = id >= 0 && !(x == NEG_INF);
+    if (has && id >= V) bad = 1.f;
+    lds.id[j] = has && id < V ? static_cast<int>(id) : -1;
+    lds.q[j] = has ? x : NEG_INF;
+    if (has) mt = fmaxf(mt, x);
+  }
+  o.mt = group_max<W>(mt, lds.slots, w);
+  float s = 0.f;
+  for (int j = w * 64 + lane; j < t.k; j += W * 64) s += __builtin_amdgcn_exp2f((lds.q[j] - o.mt) * it * LOG2E);
+  s = group_sum<W>(s, lds.slots + W, w);
+  o.bad = group_max<W>(bad, lds.slots + 2 * W, w) != 0.f;
+  o.some = s != 0.f;
+  o.lt = logf(s);
+  for (int j = w * 64 + lane; j < t.k; j += W * 64)
+    lds.q[j] = o.some ? __builtin_amdgcn_exp2f(((lds.q[j] - o.mt) * it - o.lt) * LOG2E) : 0.f;
+  group_sync<W>();
+  return o;
+}
+
+// the loss of a row from its sums and its teacher; y checked by the caller's group
+template <typename T, int W>
+__device__ __forceinline__ float distill_row_loss(const T* z, int V, const Teacher& tc, int64_t r, const Mix& mix,
+                                                  const TeacherRow& tr, TeacherLds<W>& lds, float m, float l1, float l2,
+                                                  int64_t y, int w, int lane) {
+  float kl = 0.f;
+  for (int j = w * 64 + lane; j < tc.k; j += W * 64) {
+    const int id = lds.id[j];
+    const float q = lds.q[j];
+    if (id >= 0 && !(q == 0.f))
+      kl += q * (((ld_teacher(tc, r * tc.k + j) - tr.mt) * mix.it - tr.lt) - ((to_f(z[id]) - m) * mix.it - l2));
+  }
+  kl = group_sum<W>(kl, lds.slots + 3 * W, w);
+  float loss = mix.alpha == 0.f ? 0.f : mix.alpha * mix.tau * mix.tau * kl;
+  if (mix.hard) loss += (1.f - mix.alpha) * (y >= 0 && y < V ? l1 - (to_f(z[y]) - m) : 0.f);
+  return loss;
+}
+
+// The gradient of values lo .. hi - 1 of a row: the two softmaxes everywhere first, then
+// the teacher's and the target's entries again (a repeated id writes its sum each time).
+template <typename T, int N, int U, int W>
+__device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int hi, const Teacher& tc, const Mix& mix,
+                                                 const TeacherRow& tr, const TeacherLds<W>& lds, float m, float l1,
+                                                 float l2, int64_t y, float scale, int w, int lane) {
+  const float A = tr.some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : 0.f;
+  const float B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
+  const float k1 = -l1 * LOG2E, k2 = -l2 * LOG2E, e2 = mix.it * LOG2E;
+  // one exponential where the softmaxes are the same one, or only one of them counts
+  const bool one = !mix.two;
+  const float c = A != 0.f || !mix.hard ? e2 : LOG2E, k = A != 0.f || !mix.hard ? k2 : k1, AB = A + B;
+  const bool none = A == 0.f && B == 0.f;
+  if (none && scale == scale) {
+    zero_row<T, N, W>(d, lo, hi, w, lane);
+    return;
+  }
+  const auto soft1 = [=](float x) { return AB * __builtin_amdgcn_exp2f(__builtin_fmaf(x - m, c, k)); };
+  const auto soft2 = [=](float x) {
+    const float dx = x - m;
+    return __builtin_fmaf(A, __builtin_amdgcn_exp2f(__builtin_fmaf(dx, e2, k2)),
+                          B * __builtin_amdgcn_exp2f(__builtin_fmaf(dx, LOG2E, k1)));
+  };
+  if (one) map_row<T, N, U, W>(z, d, lo, hi, w, lane, soft1);
+  else map_row<T, N, U, W>(z, d, lo, hi, w, lane, soft2);
+  group_sync<W>();
+  const auto entry = [&](int id) {
+    const float x = to_f(z[id]);
+    float g = one ? soft1(x) : soft2(x), q = 0.f;
+    for (int j = 0; j < tc.k; ++j) q += lds.id[j] == id ? lds.q[j] : 0.f;
+    g -= A * q;
+    if (id == y) g -= B;
+    from_f(d[id], g);
+  };
+  for (int j = w * 64 + lane; j < tc.k; j += W * 64)
+    if (lds.id[j] >= lo && lds.id[j] < hi) entry(lds.id[j]);
+  if (mix.hard && y >= lo && y < hi && w == 0 && lane == 0) entry(static_cast<int>(y));
+}
+
+// Sums of a row, its loss, and its gradient if dz is there, by a group of W waves.
+// row_stats: (m, log of the hard labels' sum, log of the teacher's, counted)
+template <typename T, int N, int U, int W, bool TWO>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, int64_t n_rows, int V, Teacher tc,
+                                                                   Ids targets, int64_t ignore, Mix mix, Upstream up,
+                                                                   float* __restrict__ row_loss,
+                                                                   float4* __restrict__ row_stats,
+                                                                   T* __restrict__ dz) {
+  constexpr int G = W == 1 ? 4 : 1, SECOND = TWO ? SECOND_EXP : SECOND_NONE;
+  __shared__ float slots[3 * W];
+  __shared__ TeacherLds<W> teach[G];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  if (r >= n_rows) return;
+  T* d = dz ? dz + r * V : nullptr;
+  if (!row_counts(tc, targets, ignore, r, lane)) {
+    if (w == 0 && lane == 0) {
+      row_loss[r] = 0.f;
+      row_stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (d) zero_row<T, N, W>(d, 0, V, w, lane);
+    return;
+  }
+  const T* z = row_ptr<T>(rows, r);
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  TopState no;
+  Sums a = scan_row<T, N, U, W, SECOND, false>(z, 0, V, mix.c1, mix.c2, w, lane, 0,
+                                               static_cast<TopLds<N, W>*>(nullptr), no);
+  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
+  a = group_join<SECOND, W>(a, slots, w, mix.c1, mix.c2);
+  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
+  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  if (w == 0 && lane == 0) {
+    row_loss[r] = bad ? __builtin_nanf("") : loss;
+    row_stats[r] = make_float4(a.m, l1, l2, 1.f);
+  }
+  if (d)
+    distill_row_grad<T, N, U, W>(z, d, 0, V, tc, mix, tr, lds, a.m, l1, l2, y,
+                                 bad ? __builtin_nanf("") : upstream(up, r, lane), w, lane);
+}
+
+// long rows, few of them: the sums of one part of a row ...
+template <typename T, int N, int U, int W, bool TWO>
+__global__ __launch_bounds__(64 * W) void k_distill_part(Rows rows, int V, Teacher tc, Ids targets, int64_t ignore,
+                                                         Mix mix, int parts, int part_len,
+                                                         float4* __restrict__ part_sums) {
+  constexpr int SECOND = TWO ? SECOND_EXP : SECOND_NONE;
+  __shared__ float slots[3 * W];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x / parts;
+  if (!row_counts(tc, targets, ignore, r, lane)) return;
+  const int lo = static_cast<int>(blockIdx.x % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
+  TopState no;
+  Sums a = scan_row<T, N, U, W, SECOND, false>(row_ptr<T>(rows, r), lo, hi, mix.c1, mix.c2, w, lane, 0,
+                                               static_cast<TopLds<N, W>*>(nullptr), no);
+  a = group_join<SECOND, W>(a, slots, w, mix.c1, mix.c2);
+  if (threadIdx.x == 0) part_sums[blockIdx.x] = make_float4(a.m, a.s, a.t, 0.f);
+}
+// ... joined, with the loss ...
+template <typename T, bool TWO>
+__global__ __launch_bounds__(256) void k_distill_join(Rows rows, int V, Teacher tc, Ids targets, int64_t ignore,
+                                                      Mix mix, int parts, const float4* __restrict__ part_sums,
+                                                      float* __restrict__ row_loss, float4* __restrict__ row_stats) {
+  constexpr int SECOND = TWO ? SECOND_EXP : SECOND_NONE;
+  __shared__ TeacherLds<4> lds;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t r = blockIdx.x;
-  if (!row_counts(tc, targets, ignore, r)) {
+  if (!row_counts(tc, targets, ignore, r, lane)) {
     if (threadIdx.x == 0) {
       row_loss[r] = 0.f;
       row_stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     return;
   }
-  const T* z = row_ptr<T>(rows, r);
-  const float it = 1.f / tau;
-  float m = -FLT_MAX;
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) m = fmaxf(m, to_f(z[v]));
-  m = block_max(m, red);
-  float s1 = 0.f, s2 = 0.f;
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) {
-    const float d = to_f(z[v]) - m;
-    s1 += exp_f(d);
-    s2 += exp_f(d * it);
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  Sums a;
+  if (lane < parts) {
+    const float4 v = part_sums[r * parts + lane];
+    a.m = v.x, a.s = v.y, a.t = v.z;
   }
-  const float l1 = logf(block_sum(s1, red)), l2 = logf(block_sum(s2, red));
-  float mt = -FLT_MAX;
-  for (int j = threadIdx.x; j < tc.k; j += TOK_THREADS)
-    if (teacher_has(tc, r * tc.k + j)) mt = fmaxf(mt, ld_teacher(tc, r * tc.k + j));
-  mt = block_max(mt, red);
-  float st = 0.f;
-  for (int j = threadIdx.x; j < tc.k; j += TOK_THREADS)
-    if (teacher_has(tc, r * tc.k + j)) st += exp_f((ld_teacher(tc, r * tc.k + j) - mt) * it);
-  st = block_sum(st, red);
-  const float lt = logf(st);
-  float kl = 0.f;
-  for (int j = threadIdx.x; j < tc.k; j += TOK_THREADS) {
-    if (!teacher_has(tc, r * tc.k + j)) continue;
-    const int64_t v = ld_id(tc.ids, r * tc.k + j);
-    const float lq = (ld_teacher(tc, r * tc.k + j) - mt) * it - lt, q = exp_f(lq);
-    if (v >= V) kl = __builtin_nanf("");
-    else if (!(q == 0.f)) kl += q * (lq - ((to_f(z[v]) - m) * it - l2));
-  }
-  kl = block_sum(kl, red);
+  rebase<SECOND>(a, wave_max(a.m), mix.c1, mix.c2);
+  a.s = wave_sum(a.s);
+  if constexpr (TWO) a.t = wave_sum(a.t);
+  const TeacherRow tr = teacher_row<4>(tc, r, V, mix.it, lds, w, lane);
+  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  const float loss = distill_row_loss<T, 4>(row_ptr<T>(rows, r), V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
   if (threadIdx.x == 0) {
-    float loss = alpha * tau * tau * kl;
-    if (targets.p) {
-      const int64_t y = ld_id(targets, r);
-      loss += (1.f - alpha) * (y >= 0 && y < V ? l1 - (to_f(z[y]) - m) : __builtin_nanf(""));
-    }
-    row_loss[r] = loss;
-    row_stats[r] = make_float4(m, l1, l2, 0.f);
+    row_loss[r] = tr.bad || (targets.p && (y < 0 || y >= V)) ? __builtin_nanf("") : loss;
+    row_stats[r] = make_float4(a.m, l1, l2, 1.f);
   }
 }
-
-// the gradient of one row: scale = grad_scale * upstream * norm
-template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_distill_grad(Rows rows, int V, Teacher tc, Ids targets,
-                                                              int64_t ignore, float tau, float alpha,
-                                                              const float4* __restrict__ row_stats,
-                                                              const float* __restrict__ norm,
-                                                              const float* __restrict__ up, int up_rows,
-                                                              float grad_scale, T* __restrict__ dz) {
-  __shared__ float red[TOK_THREADS];
-  const int64_t r = blockIdx.x;
+// ... and the gradient from the row's statistics
+template <typename T, int N, int U, int W>
+__global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows, int V, Teacher tc, Ids targets,
+                                                      int64_t ignore, Mix mix, Upstream up, int parts, int part_len,
+                                                      const float4* __restrict__ row_stats, T* __restrict__ dz) {
+  constexpr int G = 4 / W;
+  __shared__ TeacherLds<W> teach[G];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W, r = item / parts;
+  if (r >= n_rows) return;
+  const int lo = static_cast<int>(item % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
   T* d = dz + r * V;
-  if (!row_counts(tc, targets, ignore, r)) {
-    for (int v = threadIdx.x; v < V; v += TOK_THREADS) from_f(d[v], 0.f);
+  const float4 st = row_stats[r];
+  if (st.w == 0.f) {
+    zero_row<T, N, W>(d, lo, hi, w, lane);
+    return;
+  }
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
+  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  distill_row_grad<T, N, U, W>(row_ptr<T>(rows, r), d, lo, hi, tc, mix, tr, lds, st.x, st.y, st.z, y,
+                               bad ? __builtin_nanf("") : upstream(up, r, lane), w, lane);
+}
+
+// Rows of at most SHORT_V values, one lane per row: loss, statistics and gradient, each
+// if asked for.
+template <typename T, int M>
+__global__ __launch_bounds__(256) void k_distill_short(Rows rows, int64_t n_rows, int V, Teacher tc, Ids targets,
+                                                       int64_t ignore, Mix mix, Upstream up,
+                                                       float* __restrict__ row_loss, float4* __restrict__ row_stats,
+                                                       T* __restrict__ dz) {
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const bool live = r0 < n_rows;
+  const int64_t r = live ? r0 : n_rows - 1;
+  float scale = dz ? upstream(up, r, threadIdx.x & 63) : 0.f;  // by whole waves
+  if (!live) return;
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  float mt = -FLT_MAX;
+  bool some = false, bad = targets.p && (y < 0 || y >= V);
+  for (int j = 0; j < tc.k; ++j) {
+    if (!teacher_has(tc, r * tc.k + j)) continue;
+    some = true;
+    mt = fmaxf(mt, ld_teacher(tc, r * tc.k + j));
+    if (ld_id(tc.ids, r * tc.k + j) >= V) bad = true;
+  }
+  if (targets.p ? y == ignore : !some) {
+    if (row_loss) {
+      row_loss[r] = 0.f;
+      row_stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (dz)
+      for (int v = 0; v < V; ++v) from_f(dz[r * V + v], 0.f);
     return;
   }
   const T* z = row_ptr<T>(rows, r);
-  float scale = grad_scale;
-  if (norm) scale *= norm[0];
-  if (up) scale *= up[up_rows ? r : 0];
-  const float4 st = row_stats[r];
-  const float it = 1.f / tau;
-  float mt = -FLT_MAX;
-  for (int j = threadIdx.x; j < tc.k; j += TOK_THREADS)
-    if (teacher_has(tc, r * tc.k + j)) mt = fmaxf(mt, ld_teacher(tc, r * tc.k + j));
-  mt = block_max(mt, red);
-  float s = 0.f, bad = 0.f;
-  for (int j = threadIdx.x; j < tc.k; j += TOK_THREADS)
-    if (teacher_has(tc, r * tc.k + j)) {
-      s += exp_f((ld_teacher(tc, r * tc.k + j) - mt) * it);
-      if (ld_id(tc.ids, r * tc.k + j) >= V) bad = 1.f;
-    }
-  s = block_sum(s, red);
-  bad = block_max(bad, red);
-  const float lt = logf(s);
-  const float has = s == 0.f ? 0.f : 1.f;
-  const int64_t y = targets.p ? ld_id(targets, r) : -1;
-  if (bad != 0.f || (targets.p && (y < 0 || y >= V))) scale = __builtin_nanf("");
-  for (int v = threadIdx.x; v < V; v += TOK_THREADS) {
-    const float dv = to_f(z[v]) - st.x;
-    float soft = has != 0.f ? exp_f(dv * it - st.z) : 0.f;
-    for (int j = 0; j < tc.k; ++j)
-      if (ld_id(tc.ids, r * tc.k + j) == v && teacher_has(tc, r * tc.k + j))
-        soft -= exp_f((ld_teacher(tc, r * tc.k + j) - mt) * it - lt);
-    float g = alpha * tau * soft;
-    if (targets.p) g += (1.f - alpha) * (exp_f(dv - st.y) - (v == y ? 1.f : 0.f));
-    from_f(d[v], scale * g);
+  float x[M], q[M];
+  Sums a;
+#pragma unroll
+  for (int v = 0; v < M; ++v) {
+    x[v] = v < V ? to_f(z[v]) : NEG_INF;
+    a.m = fmaxf(a.m, x[v]);
+    q[v] = 0.f;
   }
-}
-
-// loss[0] = norm * sum of row losses (norm NULL: the sum), one fixed order
-__global__ __launch_bounds__(TOK_THREADS) void k_distill_total(const float* __restrict__ row_loss, int64_t n,
-                                                               const float* __restrict__ norm,
-                                                               float* __restrict__ loss) {
-  __shared__ float red[TOK_THREADS];
-  float s = 0.f;
-  for (int64_t r = threadIdx.x; r < n; r += TOK_THREADS) s += row_loss[r];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) loss[0] = norm ? s * norm[0] : s;
+  float s2 = 0.f;
+#pragma unroll
+  for (int v = 0; v < M; ++v) {
+    const float d = x[v] - a.m;
+    a.s += __builtin_amdgcn_exp2f(d * LOG2E);
+    s2 += __builtin_amdgcn_exp2f(d * (mix.it * LOG2E));
+  }
+  const float l1 = logf(a.s), l2 = logf(s2);
+  float st = 0.f, kl = 0.f;
+  for (int j = 0; j < tc.k; ++j)
+    if (teacher_has(tc, r * tc.k + j))
+      st += __builtin_amdgcn_exp2f((ld_teacher(tc, r * tc.k + j) - mt) * mix.it * LOG2E);
+  const float lt = logf(st);
+  for (int j = 0; j < tc.k; ++j) {
+    if (!teacher_has(tc, r * tc.k + j)) continue;
+    const int64_t id = ld_id(tc.ids, r * tc.k + j);
+    const float lq = (ld_teacher(tc, r * tc.k + j) - mt) * mix.it - lt, qj = __builtin_amdgcn_exp2f(lq * LOG2E);
+    float zi = 0.f;
+#pragma unroll
+    for (int v = 0; v < M; ++v) {
+      q[v] += v == id ? qj : 0.f;
+      zi = v == id ? x[v] : zi;
+    }
+    if (!(qj == 0.f)) kl += qj * (lq - ((zi - a.m) * mix.it - l2));
+  }
+  if (row_loss) {
+    float loss = mix.alpha == 0.f ? 0.f : mix.alpha * mix.tau * mix.tau * kl;
+    float zy = 0.f;
+#pragma unroll
+    for (int v = 0; v < M; ++v) zy = v == y ? x[v] : zy;
+    if (mix.hard) loss += (1.f - mix.alpha) * (l1 - (zy - a.m));
+    row_loss[r] = bad ? __builtin_nanf("") : loss;
+    row_stats[r] = make_float4(a.m, l1, l2, 1.f);
+  }
+  if (!dz) return;
+  if (bad) scale = __builtin_nanf("");
+  const float A = some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : bad ? scale : 0.f;
+  const float B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
+#pragma unroll
+  for (int v = 0; v < M; ++v) {
+    if (v >= V) break;
+    const float d = x[v] - a.m;
+    float g = A * (__builtin_amdgcn_exp2f(__builtin_fmaf(d, mix.it * LOG2E, -l2 * LOG2E)) - q[v]);
+    if (mix.hard) g += B * (__builtin_amdgcn_exp2f(__builtin_fmaf(d, LOG2E, -l1 * LOG2E)) - (v == y ? 1.f : 0.f));
+    from_f(dz[r * V + v], g);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -924,6 +1269,34 @@ extern "C" int ghm_token_logprobs(const void* logits, int dtype, int64_t n_inner
   return ghm_launch_status();
 }
 
+namespace {
+template <typename T, int N, int U, int W>
+void launch_score_bwd(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreGrad& g,
+                      const Split& p, T* dz, hipStream_t s) {
+  constexpr int G = 4 / W;
+  hipLaunchKernelGGL((k_score_bwd<T, N, U, W>), dim3(static_cast<unsigned>((rows * p.parts + G - 1) / G)), dim3(256), 0,
+                     s, m, rows, V, t, ignore, g, p.parts, p.len, dz);
+}
+template <typename T>
+void score_bwd_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreGrad& g, void* dlogits,
+                   hipStream_t s) {
+  constexpr int N = Vec<T>::N;
+  T* dz = static_cast<T*>(dlogits);
+  const Split p = map_split(rows, V);
+  if (V <= SHORT_V) {
+    const dim3 gr(static_cast<unsigned>((rows + 255) / 256));
+    if (V <= 12) hipLaunchKernelGGL((k_score_bwd_short<T, 12>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
+    else hipLaunchKernelGGL((k_score_bwd_short<T, SHORT_V>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
+  } else if (V <= 512) {
+    launch_score_bwd<T, 1, 8, 1>(m, rows, V, t, ignore, g, p, dz, s);
+  } else if (V <= 2048) {
+    launch_score_bwd<T, N, 4, 1>(m, rows, V, t, ignore, g, p, dz, s);
+  } else {
+    launch_score_bwd<T, N, 4, 4>(m, rows, V, t, ignore, g, p, dz, s);
+  }
+}
+}  // namespace
+
 extern "C" int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_inner, int64_t s_outer,
                                       int64_t s_inner, int64_t rows, int64_t V, const void* targets, int id_bits,
                                       int64_t ignore_index, int top_k, const int64_t* top_id, const float* stats,
@@ -936,11 +1309,9 @@ extern "C" int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_i
                           (!d_top || (top_id && top_k >= 1))), "null pointer");
   if (rows == 0) return GHM_OK;
   const Rows m{logits, n_inner, s_outer, s_inner};
-  const Ids t{targets, id_bits};
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_score_bwd<T>, dim3(static_cast<unsigned>(rows)), dim3(TOK_THREADS), 0,
-                                         ghm_stream(stream), m, static_cast<int>(V), t, ignore_index,
-                                         d_top ? top_k : 0, top_id, reinterpret_cast<const float2*>(stats), entropy,
-                                         d_logprob, d_entropy, d_top, static_cast<T*>(dlogits)));
+  const ScoreGrad g{top_id, reinterpret_cast<const float2*>(stats), entropy, d_logprob, d_entropy, d_top, top_k};
+  TOK_DISPATCH(dtype, score_bwd_any<T>(m, rows, static_cast<int>(V), Ids{targets, id_bits}, ignore_index, g, dlogits,
+                                       ghm_stream(stream)));
   return ghm_launch_status();
 }
 
@@ -952,9 +1323,107 @@ extern "C" int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_i
   GHM_CHECK(temperature > 0.f && temperature <= FLT_MAX, "temperature");                                        \
   GHM_CHECK(alpha >= 0.f && alpha <= 1.f && (targets || alpha == 1.f), "alpha (0 .. 1; below 1 needs targets)")
 
+namespace {
+struct Distill {
+  Rows m;
+  int64_t rows;
+  int V;
+  Teacher tc;
+  Ids t;
+  int64_t ignore;
+  Mix mix;
+  float* row_loss;
+  float4* stats;
+  hipStream_t s;
+};
+// ws: counts [64] int, range sums [64] float2, then a part's sums each
+constexpr int64_t DISTILL_WS_HEAD = MAX_COUNTS * 4 + MAX_COUNTS * 8;
+
+inline Mix make_mix(bool targets, float tau, float alpha) {
+  Mix x;
+  x.tau = tau;
+  x.it = 1.f / tau;
+  x.alpha = alpha;
+  x.hard = targets && alpha < 1.f;
+  x.two = x.hard && alpha > 0.f && tau != 1.f;
+  x.c1 = x.hard ? LOG2E : LOG2E * x.it;
+  x.c2 = LOG2E * x.it;
+  return x;
+}
+
+template <typename T, int N, int U, int W>
+void launch_distill(const Distill& a, const Upstream& up, T* dz) {
+  constexpr int G = W == 1 ? 4 : 1;
+  const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
+  if (a.mix.two)
+    hipLaunchKernelGGL((k_distill<T, N, U, W, true>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       a.row_loss, a.stats, dz);
+  else
+    hipLaunchKernelGGL((k_distill<T, N, U, W, false>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       a.row_loss, a.stats, dz);
+}
+template <typename T, int N, int U, int W>
+void launch_distill_grad(const Distill& a, const Upstream& up, const Split& p, T* dz) {
+  constexpr int G = 4 / W;
+  hipLaunchKernelGGL((k_distill_grad<T, N, U, W>), dim3(static_cast<unsigned>((a.rows * p.parts + G - 1) / G)), dim3(256),
+                     0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up, p.parts, p.len, a.stats, dz);
+}
+template <typename T>
+void distill_short(const Distill& a, const Upstream& up, float* row_loss, T* dz) {
+  const dim3 g(static_cast<unsigned>((a.rows + 255) / 256)), b(256);
+  if (a.V <= 12)
+    hipLaunchKernelGGL((k_distill_short<T, 12>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       row_loss, a.stats, dz);
+  else
+    hipLaunchKernelGGL((k_distill_short<T, SHORT_V>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       row_loss, a.stats, dz);
+}
+template <typename T>
+void distill_grad_any(const Distill& a, const Upstream& up, T* dz) {
+  constexpr int N = Vec<T>::N;
+  const Split p = map_split(a.rows, a.V);
+  if (a.V <= SHORT_V) distill_short<T>(a, up, nullptr, dz);
+  else if (a.V <= 512) launch_distill_grad<T, 1, 8, 1>(a, up, p, dz);
+  else if (a.V <= 2048) launch_distill_grad<T, N, 4, 1>(a, up, p, dz);
+  else launch_distill_grad<T, N, 4, 4>(a, up, p, dz);
+}
+template <typename T>
+void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) {
+  constexpr int N = Vec<T>::N;
+  T* dz = static_cast<T*>(dlogits);
+  const Split p = row_split(a.rows, a.V);
+  if (a.V <= SHORT_V) {
+    distill_short<T>(a, up, a.row_loss, dz);
+  } else if (a.V <= 512) {
+    launch_distill<T, 1, 8, 1>(a, up, dz);
+  } else if (a.V <= 2048) {
+    launch_distill<T, N, 4, 1>(a, up, dz);
+  } else if (p.parts == 1) {
+    launch_distill<T, N, 4, 8>(a, up, dz);
+  } else {
+    float4* sums = reinterpret_cast<float4*>(static_cast<char*>(ws) + DISTILL_WS_HEAD);
+    const dim3 g(static_cast<unsigned>(a.rows * p.parts)), g1(static_cast<unsigned>(a.rows));
+    if (a.mix.two) {
+      hipLaunchKernelGGL((k_distill_part<T, N, 4, 8, true>), g, dim3(512), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix,
+                         p.parts, p.len, sums);
+      hipLaunchKernelGGL((k_distill_join<T, true>), g1, dim3(256), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
+                         sums, a.row_loss, a.stats);
+    } else {
+      hipLaunchKernelGGL((k_distill_part<T, N, 4, 8, false>), g, dim3(512), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix,
+                         p.parts, p.len, sums);
+      hipLaunchKernelGGL((k_distill_join<T, false>), g1, dim3(256), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
+                         sums, a.row_loss, a.stats);
+    }
+    if (dz) distill_grad_any<T>(a, up, dz);
+  }
+}
+}  // namespace
+
 extern "C" int64_t ghm_distill_ws(int64_t rows, int64_t V, int dtype) {
-  (void)rows; (void)V; (void)dtype;
-  return 0;
+  (void)dtype;
+  if (rows <= 0 || V <= 0) return DISTILL_WS_HEAD;
+  const Split p = row_split(rows, V);
+  return DISTILL_WS_HEAD + (p.parts == 1 ? 0 : rows * p.parts * 16);
 }
 
 extern "C" int ghm_distill(const void* logits, int dtype, int64_t n_inner, int64_t s_outer, int64_t s_inner,
@@ -966,25 +1435,31 @@ extern "C" int ghm_distill(const void* logits, int dtype, int64_t n_inner, int64
   GHM_CHECK(reduction >= 0 && reduction <= 2, "reduction (0 none, 1 mean, 2 sum)");
   GHM_CHECK((reduction == 0 || loss) && (reduction != 1 || norm), "null pointer");
   GHM_CHECK(rows == 0 || (logits && top_ids && top_logits && row_loss && stats), "null pointer");
-  GHM_CHECK(ws_bytes >= ghm_distill_ws(rows, V, dtype), "workspace too small");
-  (void)ws;
-  hipStream_t s = ghm_stream(stream);
-  const Rows m{logits, n_inner, s_outer, s_inner};
-  const Teacher tc{{top_ids, id_bits}, top_logits, t_dtype, k};
-  const Ids t{targets, target_bits};
-  float4* st = reinterpret_cast<float4*>(stats);
-  const float* nm = reduction == 1 ? norm : nullptr;
-  const dim3 g(static_cast<unsigned>(rows)), b(TOK_THREADS);
-  if (nm) hipLaunchKernelGGL(k_distill_count, dim3(1), b, 0, s, tc, t, ignore_index, rows, norm);
-  if (rows) {
-    TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_distill_rows<T>, g, b, 0, s, m, static_cast<int>(V), tc, t, ignore_index,
-                                           temperature, alpha, row_loss, st));
-    if (dlogits)
-      TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_distill_grad<T>, g, b, 0, s, m, static_cast<int>(V), tc, t,
-                                             ignore_index, temperature, alpha, st, nm, nullptr, 0, grad_scale,
-                                             static_cast<T*>(dlogits)));
+  GHM_CHECK(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "stats (16-byte aligned)");
+  GHM_CHECK(ws && ws_bytes >= ghm_distill_ws(rows, V, dtype) && reinterpret_cast<uintptr_t>(ws) % 16 == 0,
+            "workspace (too small, or not 16-byte aligned)");
+  const Distill a{{logits, n_inner, s_outer, s_inner}, rows, static_cast<int>(V), {{top_ids, id_bits}, top_logits, t_dtype, k},
+                  {targets, target_bits}, ignore_index, make_mix(targets != nullptr, temperature, alpha), row_loss,
+                  reinterpret_cast<float4*>(stats), ghm_stream(stream)};
+  int* counts = static_cast<int*>(ws);
+  float2* ranges = reinterpret_cast<float2*>(counts + MAX_COUNTS);
+  Upstream up{nullptr, 0, nullptr, nullptr, 0, grad_scale};
+  if (rows && dlogits && reduction == 1) {  // the gradient needs the number of counted rows first
+    const int nb = static_cast<int>((rows + 1023) / 1024 < MAX_COUNTS ? (rows + 1023) / 1024 : MAX_COUNTS);
+    hipLaunchKernelGGL(k_distill_count, dim3(nb), dim3(256), 0, a.s, a.tc, a.t, ignore_index, rows, (rows + nb - 1) / nb,
+                       counts);
+    up.counts = counts;
+    up.n_counts = nb;
   }
-  if (reduction) hipLaunchKernelGGL(k_distill_total, dim3(1), b, 0, s, row_loss, rows, nm, loss);
+  if (rows) TOK_DISPATCH(dtype, distill_any<T>(a, up, dlogits, ws));
+  if (reduction) {
+    // one block up to 16,384 rows, ranges of that many (at most 64) above
+    const int nb = static_cast<int>((rows + 16383) / 16384 < 1 ? 1 : (rows + 16383) / 16384 < MAX_COUNTS ? (rows + 16383) / 16384 : MAX_COUNTS);
+    hipLaunchKernelGGL(k_distill_total, dim3(nb), dim3(1024), 0, a.s, row_loss, a.stats, rows, (rows + nb - 1) / nb,
+                       ranges, reduction == 1, loss, norm);
+    if (nb > 1)
+      hipLaunchKernelGGL(k_distill_total2, dim3(1), dim3(64), 0, a.s, ranges, nb, reduction == 1, loss, norm);
+  }
   return ghm_launch_status();
 }
 
@@ -995,14 +1470,13 @@ extern "C" int ghm_distill_bwd(const void* logits, int dtype, int64_t n_inner, i
                                const float* d_loss, int d_rows, void* dlogits, void* stream) {
   DISTILL_CHECK();
   GHM_CHECK(rows == 0 || (logits && top_ids && top_logits && stats && d_loss && dlogits), "null pointer");
+  GHM_CHECK(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "stats (16-byte aligned)");
   if (rows == 0) return GHM_OK;
-  const Rows m{logits, n_inner, s_outer, s_inner};
-  const Teacher tc{{top_ids, id_bits}, top_logits, t_dtype, k};
-  const Ids t{targets, target_bits};
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_distill_grad<T>, dim3(static_cast<unsigned>(rows)), dim3(TOK_THREADS), 0,
-                                         ghm_stream(stream), m, static_cast<int>(V), tc, t, ignore_index, temperature,
-                                         alpha, reinterpret_cast<const float4*>(stats), norm, d_loss, d_rows, 1.f,
-                                         static_cast<T*>(dlogits)));
+  const Distill a{{logits, n_inner, s_outer, s_inner}, rows, static_cast<int>(V), {{top_ids, id_bits}, top_logits, t_dtype, k},
+                  {targets, target_bits}, ignore_index, make_mix(targets != nullptr, temperature, alpha), nullptr,
+                  reinterpret_cast<float4*>(const_cast<float*>(stats)), ghm_stream(stream)};
+  const Upstream up{nullptr, 0, norm, d_loss, d_rows, 1.f};
+  TOK_DISPATCH(dtype, distill_grad_any<T>(a, up, static_cast<T*>(dlogits)));
   return ghm_launch_status();
 }
 
