@@ -14,7 +14,6 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NEG_INF = -__builtin_inff();
-constexpr int TOK_THREADS = 256;
 
 struct bf16_t { uint16_t u; };
 struct f16_t { _Float16 h; };
@@ -1166,28 +1165,304 @@ __global__ __launch_bounds__(256) void k_distill_short(Rows rows, int64_t n_rows
 }
 
 // ---------------------------------------------------------------------------
-// Scaled embedding: out_i = scale W[tok_i]; dW_v = scale sum_{i: tok_i = v} dout_i,
-// summed in f32 in ascending i and rounded once.
+// Scaled embedding: out_i = scale W[tok_i].
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_embed_rows(Ids tok, const T* __restrict__ w, int64_t w_stride,
-                                                            float scale, T* __restrict__ out, int64_t V, int64_t D) {
-  const int64_t i = blockIdx.x, v = ld_id(tok, i);
-  const bool ok = v >= 0 && v < V;
-  for (int64_t c = threadIdx.x; c < D; c += TOK_THREADS)
-    from_f(out[i * D + c], ok ? to_f(w[v * w_stride + c]) * scale : __builtin_nanf(""));
+// up to VE values of a row from column c on (fewer at its end; the rest 0)
+template <typename T, int VE>
+__device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&x)[VE]) {
+  if (c + VE <= D) {
+    load_vec<VE>(row + c, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) x[i] = c + i < D ? to_f(row[c + i]) : 0.f;
+  }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&x)[VE]) {
+  if (c + VE <= D) {
+    store_vec<VE>(row + c, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (c + i < D) from_f(row[c + i], x[i]);
+  }
 }
 
+// A block takes `per` rows of `vecs` vectors; lanes take vectors in turn.
 template <typename T>
-__global__ __launch_bounds__(TOK_THREADS) void k_embed_rows_bwd(Ids tok, const T* __restrict__ dout, int64_t d_stride,
-                                                                float scale, int64_t padding, T* __restrict__ dw,
-                                                                int64_t N, int64_t D) {
-  const int64_t v = blockIdx.x, c = static_cast<int64_t>(blockIdx.y) * TOK_THREADS + threadIdx.x;
+__global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict__ weight, int64_t w_stride,
+                                                    float scale, T* __restrict__ out, int64_t N, int64_t V, int D,
+                                                    int vecs, int per) {
+  constexpr int VE = Vec<T>::N, U = 4;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per;
+  const int n = static_cast<int>(N - i0 < per ? N - i0 : per) * vecs;
+  for (int t0 = threadIdx.x; t0 < n; t0 += 256 * U) {
+    float x[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + 256 * u;
+      if (t >= n) break;
+      const int64_t v = ld_id(tok, i0 + t / vecs);
+      if (v >= 0 && v < V) {
+        load_cols<T, VE>(weight + v * w_stride, t % vecs * VE, D, x[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[u][i] = __builtin_nanf("");
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + 256 * u;
+      if (t >= n) break;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) x[u][i] *= scale;
+      store_cols<T, VE>(out + (i0 + t / vecs) * D, t % vecs * VE, D, x[u]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Its gradient dW_v = scale sum_{i: tok_i = v} dout_i.  The positions are sorted by token
+// (stable radix sort, so a token's positions stay in order); chunks of the sorted list are
+// summed in f32, a token that crosses chunks through partial rows joined in order; table
+// rows without a token are written 0 beside it.  No atomics on values: a fixed order.
+// ---------------------------------------------------------------------------
+constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_ROUNDS = 8;
+constexpr int SORT_TILES = 128;  // up to this many tiles a block sums their counts itself
+
+// the sorted key of position i: its token; `none` for a token that gets no gradient
+__device__ __forceinline__ uint32_t sort_key(const Ids& tok, int64_t i, int64_t pad, uint32_t none) {
+  const int64_t v = ld_id(tok, i);
+  return v >= 0 && v < none && v != pad ? static_cast<uint32_t>(v) : none;
+}
+struct SortIn {  // the first pass reads tokens, later ones the previous pass's keys and positions
+  Ids tok;
+  const uint32_t *key, *pos;
+  int64_t pad;
+  uint32_t none;
+};
+__device__ __forceinline__ uint32_t sort_in(const SortIn& in, int64_t i) {
+  return in.key ? in.key[i] : sort_key(in.tok, i, in.pad, in.none);
+}
+
+// counts[tile][digit]; the first pass also clears the table of rows that have a token
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_sort_count(SortIn in, int64_t N, int shift, uint32_t* __restrict__ counts,
+                                                       uint32_t* __restrict__ used, int64_t used_words) {
+  __shared__ uint32_t bins[SORT_BINS];
+  constexpr int TILE = 64 * W * SORT_ROUNDS;
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) bins[d] = 0;
+  if (used)
+    for (int64_t j = static_cast<int64_t>(blockIdx.x) * 64 * W + threadIdx.x; j < used_words;
+         j += static_cast<int64_t>(gridDim.x) * 64 * W)
+      used[j] = 0;
+  __syncthreads();
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * TILE;
+#pragma unroll
+  for (int q = 0; q < SORT_ROUNDS; ++q) {
+    const int64_t i = i0 + q * 64 * W + threadIdx.x;
+    if (i < N) atomicAdd(&bins[(sort_in(in, i) >> shift) & (SORT_BINS - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d] = bins[d];
+}
+// many tiles: counts become, digit by digit, the sums over the tiles before; the totals follow
+__global__ __launch_bounds__(64) void k_sort_scan(uint32_t* __restrict__ counts, int64_t tiles) {
+  uint32_t* c = counts + blockIdx.x * 64 + threadIdx.x;
+  uint32_t s = 0;
+#pragma unroll 8
+  for (int64_t t = 0; t < tiles; ++t) {
+    const uint32_t v = c[t * SORT_BINS];
+    c[t * SORT_BINS] = s;
+    s += v;
+  }
+  c[tiles * SORT_BINS] = s;
+}
+// Positions go to: start of the digit + the digit's count in earlier tiles + in earlier
+// waves + in this wave's earlier rounds + among lower lanes.  A wave takes 64 * SORT_ROUNDS
+// consecutive positions, so the sort is stable.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, int shift,
+                                                         const uint32_t* __restrict__ counts, int tiles, int scanned,
+                                                         uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
+                                                         uint8_t* __restrict__ used) {
+  __shared__ uint32_t wbins[W][SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  for (int d = lane; d < SORT_BINS; d += 64) wbins[w][d] = 0;
+  // digit totals and the counts of earlier tiles; then an exclusive scan over the digits
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
+    uint32_t before = 0, all = 0;
+    if (scanned) {
+      before = counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d];
+      all = counts[static_cast<int64_t>(tiles) * SORT_BINS + d];
+    } else {
+#pragma unroll 8
+      for (int t = 0; t < tiles; ++t) {
+        const uint32_t c = counts[t * SORT_BINS + d];
+        before += t < static_cast<int>(blockIdx.x) ? c : 0;
+        all += c;
+      }
+    }
+    uint32_t inc = all;  // 64 consecutive digits per wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up(inc, o, 64);
+      inc += lane >= o ? up : 0;
+    }
+    if (lane == 63) wsum[d >> 6] = inc;
+    base[d] = inc - all + before;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
+    uint32_t s = base[d];
+    for (int j = 0; j < d >> 6; ++j) s += wsum[j];
+    base[d] = s;
+  }
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * W + w) * 64 * SORT_ROUNDS + lane;
+  uint32_t key[SORT_ROUNDS], at[SORT_ROUNDS], pos[SORT_ROUNDS];
+#pragma unroll
+  for (int q = 0; q < SORT_ROUNDS; ++q) {
+    const int64_t i = i0 + q * 64;
+    key[q] = i < N ? sort_in(in, i) : 0;
+    pos[q] = i < N && in.pos ? in.pos[i] : static_cast<uint32_t>(i);
+  }
+#pragma unroll
+  for (int q = 0; q < SORT_ROUNDS; ++q) {
+    const bool live = i0 + q * 64 < N;
+    const uint32_t d = (key[q] >> shift) & (SORT_BINS - 1);
+    uint64_t same = __ballot(live);
+#pragma unroll
+    for (int bit = 0; bit < SORT_BITS; ++bit) {
+      const uint64_t m = __ballot((d >> bit) & 1);
+      same &= (d >> bit) & 1 ? m : ~m;
+    }
+    const uint64_t lower = same & ((uint64_t(1) << lane) - 1);
+    at[q] = wbins[w][d] + __popcll(lower);
+    wave_fence();
+    if (live && lower == 0) wbins[w][d] += __popcll(same);
+    wave_fence();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < SORT_ROUNDS; ++q) {
+    if (i0 + q * 64 >= N) break;
+    const uint32_t d = (key[q] >> shift) & (SORT_BINS - 1);
+    uint32_t to = base[d] + at[q];
+    for (int j = 0; j < w; ++j) to += wbins[j][d];
+    key_out[to] = key[q];
+    pos_out[to] = pos[q];
+    if (used && key[q] != in.none) used[key[q]] = 1;
+  }
+}
+
+// Chunk c of the sorted list, columns col .. col + VE - 1 per lane; `lpr` lanes per row,
+// 64 / lpr chunks per wave.  A token inside the chunk is finished here; one that goes on
+// from the chunk before leaves its sum in parts[c][0], one that begins here and goes on
+// after it in parts[c][1].  Blocks past the chunks clear table rows without a token.
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
+                                                    uint32_t none, const T* __restrict__ dout, int64_t d_stride,
+                                                    float scale, T* __restrict__ dw, int64_t N, int D, int chunk,
+                                                    int64_t chunks, int slices, int lpr, int64_t sum_blocks,
+                                                    float* __restrict__ parts, const uint8_t* __restrict__ used,
+                                                    int64_t V, int rows_per_block) {
+  constexpr int VE = Vec<T>::N, U = 8;
+  if (blockIdx.x >= sum_blocks) {
+    const int64_t v0 = (blockIdx.x - sum_blocks) * rows_per_block;
+    const int64_t v1 = v0 + rows_per_block < V ? v0 + rows_per_block : V;
+    const float zero[VE] = {};
+    for (int64_t v = v0 + (threadIdx.x >> 6); v < v1; v += 4)
+      if (!used[v])
+        for (int c = (threadIdx.x & 63) * VE; c < D; c += 64 * VE) store_cols<T, VE>(dw + v * D, c, D, zero);
+    return;
+  }
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / lpr;
+  const int64_t c = group / slices;
+  const int col = (static_cast<int>(group % slices) * lpr + threadIdx.x % lpr) * VE;
+  if (c >= chunks || col >= D) return;
+  const int64_t lo = c * chunk, hi = lo + chunk < N ? lo + chunk : N;
+  uint32_t cur = key[lo];
+  bool left = lo > 0 && key[lo - 1] == cur;
+  float acc[VE] = {};
+  const auto flush = [&](bool right) {
+    if (cur == none) return;
+    if (left || right) {
+      float* o = parts + (c * 2 + (left ? 0 : 1)) * D;
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (col + i < D) o[col + i] = acc[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] *= scale;
+      store_cols<T, VE>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
+    }
+  };
+  for (int64_t i = lo; i < hi; i += U) {
+    uint32_t k[U];
+    float x[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = i + u < hi ? key[i + u] : none;
+      if (k[u] != none) load_cols<T, VE>(dout + static_cast<int64_t>(pos[i + u]) * d_stride, col, D, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= hi) break;
+      if (k[u] != cur) {
+        flush(false);
+        cur = k[u];
+        left = false;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = 0.f;
+      }
+      if (cur != none) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] += x[u][e];
+      }
+    }
+  }
+  flush(hi < N && key[hi] == cur);
+}
+
+// A token that begins in chunk c and goes on: parts[c][1] + parts[c + 1][0] + ... in order,
+// a quarter of them per wave.
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, uint32_t none, float scale,
+                                                    T* __restrict__ dw, int64_t N, int D, int chunk, int64_t chunks,
+                                                    const float* __restrict__ parts) {
+  __shared__ float red[4][64];
+  const int64_t c = blockIdx.x, lo = c * chunk, hi = lo + chunk;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.y * 64 + lane;
+  if (hi >= N) return;
+  const uint32_t k = key[hi];
+  if (k == none || key[hi - 1] != k || (lo > 0 && key[lo - 1] == k)) return;
+  int64_t n = 1;  // chunks c .. c + n - 1 hold the token
+  for (int64_t j = c + 1 + lane;; j += 64) {
+    const uint64_t m = __ballot(j < chunks && key[j * chunk] == k);
+    if (m == ~uint64_t(0)) {
+      n += 64;
+      continue;
+    }
+    n += __builtin_ctzll(~m);
+    break;
+  }
+  const int64_t q = (n + 3) / 4, a = w * q, b = a + q < n ? a + q : n;
   float s = 0.f;
-  if (v != padding)
-    for (int64_t i = 0; i < N; ++i)
-      if (ld_id(tok, i) == v && c < D) s += to_f(dout[i * d_stride + c]);
-  if (c < D) from_f(dw[v * D + c], s * scale);
+  if (col < D) {
+#pragma unroll 8
+    for (int64_t j = a; j < b; ++j) s += parts[((c + j) * 2 + (j == 0 ? 1 : 0)) * D + col];
+  }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && col < D)
+    from_f(dw[static_cast<int64_t>(k) * D + col], (((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane]) * scale);
+}
+
+// no token at all: every table row is 0
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_zero(T* __restrict__ dw, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    from_f(dw[i], 0.f);
 }
 
 inline bool ids_ok(int bits) { return bits == 8 || bits == 32 || bits == 64; }
@@ -1445,7 +1720,7 @@ extern "C" int ghm_distill(const void* logits, int dtype, int64_t n_inner, int64
   float2* ranges = reinterpret_cast<float2*>(counts + MAX_COUNTS);
   Upstream up{nullptr, 0, nullptr, nullptr, 0, grad_scale};
   if (rows && dlogits && reduction == 1) {  // the gradient needs the number of counted rows first
-    const int nb = static_cast<int>((rows + 1023) / 1024 < MAX_COUNTS ? (rows + 1023) / 1024 : MAX_COUNTS);
+    const int nb = static_cast<int>((rows + 255) / 256 < MAX_COUNTS ? (rows + 255) / 256 : MAX_COUNTS);
     hipLaunchKernelGGL(k_distill_count, dim3(nb), dim3(256), 0, a.s, a.tc, a.t, ignore_index, rows, (rows + nb - 1) / nb,
                        counts);
     up.counts = counts;
@@ -1482,8 +1757,8 @@ extern "C" int ghm_distill_bwd(const void* logits, int dtype, int64_t n_inner, i
 
 #define EMBED_CHECK()                                                                                              \
   GHM_CHECK(dtype_ok(dtype) && ids_ok(id_bits), "dtype (0 f32, 1 bf16, 2 f16), id_bits (8, 32, 64)");              \
-  GHM_CHECK(N >= 0 && N < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31) && D >= 1 && D < (int64_t(1) << 24), \
-            "shape (N, V < 2^31, D < 2^24)")
+  GHM_CHECK(N >= 0 && N < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31) && D >= 1 && D <= (int64_t(1) << 20), \
+            "shape (N, V < 2^31, D <= 2^20)")
 
 extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* weight, int dtype, int64_t w_stride,
                                   float scale, void* out, int64_t N, int64_t V, int64_t D, void* stream) {
@@ -1491,15 +1766,106 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
   GHM_CHECK(w_stride >= 0, "row stride");
   GHM_CHECK(N == 0 || (tokens && weight && out), "null pointer");
   if (N == 0) return GHM_OK;
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_rows<T>, dim3(static_cast<unsigned>(N)), dim3(TOK_THREADS), 0,
+  const int ve = dtype == 0 ? 4 : 8, vecs = static_cast<int>((D + ve - 1) / ve);
+  const int per = vecs >= 1024 ? 1 : 1024 / vecs;
+  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_rows<T>, dim3(static_cast<unsigned>((N + per - 1) / per)), dim3(256), 0,
                                          ghm_stream(stream), Ids{tokens, id_bits}, static_cast<const T*>(weight),
-                                         w_stride, scale, static_cast<T*>(out), V, D));
+                                         w_stride, scale, static_cast<T*>(out), N, V, static_cast<int>(D), vecs, per));
   return ghm_launch_status();
 }
 
+namespace {
+struct EmbedPlan {
+  int W, passes, bits, chunk, slices, lpr;
+  int64_t tiles, chunks, used_words;
+  int64_t key[2], pos[2], counts, used, parts, bytes;  // byte offsets in the workspace
+};
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
+  EmbedPlan p;
+  int bits = 1;
+  while (bits < 32 && (int64_t(1) << bits) <= V) ++bits;  // keys 0 .. V
+  p.passes = (bits + SORT_BITS - 1) / SORT_BITS;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  p.W = N <= 65536 ? 4 : 16;
+  const int64_t tile = 64 * p.W * SORT_ROUNDS;
+  p.tiles = (N + tile - 1) / tile;
+  p.lpr = 1;
+  while (p.lpr < 64 && p.lpr * ve < D) p.lpr *= 2;
+  p.slices = static_cast<int>((D + p.lpr * ve - 1) / (p.lpr * ve));
+  const int64_t want = N * p.slices / (4096 * (64 / p.lpr));
+  p.chunk = 16;
+  while (p.chunk < 256 && p.chunk < want) p.chunk *= 2;
+  p.chunks = (N + p.chunk - 1) / p.chunk;
+  p.used_words = (V + 3) / 4;
+  int64_t at = 0;
+  for (int i = 0; i < 2; ++i) {
+    p.key[i] = at, at += up256(N * 4);
+    p.pos[i] = at, at += up256(N * 4);
+  }
+  p.counts = at, at += up256((p.tiles + 1) * SORT_BINS * 4);
+  p.used = at, at += up256(p.used_words * 4);
+  p.parts = at, at += up256(p.chunks * 2 * D * 4);
+  p.bytes = at;
+  return p;
+}
+
+template <int W>
+void launch_sort(const EmbedPlan& p, const Ids& tok, int64_t pad, int64_t N, int64_t V, char* ws, hipStream_t s) {
+  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
+  uint32_t* used = reinterpret_cast<uint32_t*>(ws + p.used);
+  const dim3 g(static_cast<unsigned>(p.tiles)), b(64 * W);
+  const int scanned = p.tiles > SORT_TILES;
+  for (int i = 0; i < p.passes; ++i) {
+    SortIn in{tok, nullptr, nullptr, pad, static_cast<uint32_t>(V)};
+    if (i > 0) {
+      in.key = reinterpret_cast<uint32_t*>(ws + p.key[(i - 1) & 1]);
+      in.pos = reinterpret_cast<uint32_t*>(ws + p.pos[(i - 1) & 1]);
+    }
+    // a digit has SORT_BITS bits; the passes are p.bits apart, so digits may overlap by
+    // bits that an earlier pass has sorted already
+    hipLaunchKernelGGL(k_sort_count<W>, g, b, 0, s, in, N, i * p.bits, counts, i == 0 ? used : nullptr, p.used_words);
+    if (scanned) hipLaunchKernelGGL(k_sort_scan, dim3(SORT_BINS / 64), dim3(64), 0, s, counts, p.tiles);
+    hipLaunchKernelGGL(k_sort_scatter<W>, g, b, 0, s, in, N, i * p.bits, counts, static_cast<int>(p.tiles), scanned,
+                       reinterpret_cast<uint32_t*>(ws + p.key[i & 1]), reinterpret_cast<uint32_t*>(ws + p.pos[i & 1]),
+                       i == 0 ? reinterpret_cast<uint8_t*>(used) : nullptr);
+  }
+}
+template <typename T>
+void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale, int64_t pad, T* dw, int64_t N, int64_t V,
+                   int D, char* ws, hipStream_t s) {
+  if (N == 0) {
+    const int64_t n = V * D, blocks = (n + 1023) / 1024;
+    hipLaunchKernelGGL(k_embed_zero<T>, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, dw, n);
+    return;
+  }
+  const EmbedPlan p = embed_plan(N, V, D, Vec<T>::N);
+  if (p.W == 4) launch_sort<4>(p, tok, pad, N, V, ws, s);
+  else launch_sort<16>(p, tok, pad, N, V, ws, s);
+  const uint32_t* key = reinterpret_cast<uint32_t*>(ws + p.key[(p.passes - 1) & 1]);
+  const uint32_t* pos = reinterpret_cast<uint32_t*>(ws + p.pos[(p.passes - 1) & 1]);
+  float* parts = reinterpret_cast<float*>(ws + p.parts);
+  const uint8_t* used = reinterpret_cast<uint8_t*>(ws + p.used);
+  const int64_t sum_blocks = (p.chunks * p.slices * p.lpr + 255) / 256;
+  // about 64 KiB of table rows per clearing block, at most 2^20 of them
+  int64_t rpb = 65536 / (D * static_cast<int64_t>(sizeof(T)));
+  if (rpb < 4) rpb = 4;
+  if (rpb > 4096) rpb = 4096;
+  while ((V + rpb - 1) / rpb > (1 << 20)) rpb *= 2;
+  const int64_t zero_blocks = (V + rpb - 1) / rpb;
+  hipLaunchKernelGGL(k_embed_sums<T>, dim3(static_cast<unsigned>(sum_blocks + zero_blocks)), dim3(256), 0, s, key, pos,
+                     static_cast<uint32_t>(V), dout, d_stride, scale, dw, N, D, p.chunk, p.chunks, p.slices, p.lpr,
+                     sum_blocks, parts, used, V, static_cast<int>(rpb));
+  if (p.chunks > 1)
+    hipLaunchKernelGGL(k_embed_join<T>, dim3(static_cast<unsigned>(p.chunks - 1), static_cast<unsigned>((D + 63) / 64)),
+                       dim3(256), 0, s, key, static_cast<uint32_t>(V), scale, dw, N, D, p.chunk, p.chunks, parts);
+}
+}  // namespace
+
 extern "C" int64_t ghm_embed_rows_bwd_ws(int64_t N, int64_t V, int64_t D) {
-  (void)N; (void)V; (void)D;
-  return 0;
+  if (N <= 0 || V <= 0 || D <= 0) return 0;
+  const int64_t a = embed_plan(N, V, D, 4).bytes, b = embed_plan(N, V, D, 8).bytes;
+  return a > b ? a : b;
 }
 
 extern "C" int ghm_embed_rows_bwd(const void* tokens, int id_bits, const void* dout, int dtype, int64_t d_stride,
@@ -1508,12 +1874,11 @@ extern "C" int ghm_embed_rows_bwd(const void* tokens, int id_bits, const void* d
   EMBED_CHECK();
   GHM_CHECK(d_stride >= 0 && padding_idx >= -1 && padding_idx < V, "row stride, padding_idx (-1 .. V - 1)");
   GHM_CHECK(dweight && (N == 0 || (tokens && dout)), "null pointer");
-  GHM_CHECK(ws_bytes >= ghm_embed_rows_bwd_ws(N, V, D), "workspace too small");
-  (void)ws;
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_rows_bwd<T>,
-                                         dim3(static_cast<unsigned>(V), static_cast<unsigned>((D + TOK_THREADS - 1) / TOK_THREADS)),
-                                         dim3(TOK_THREADS), 0, ghm_stream(stream), Ids{tokens, id_bits},
-                                         static_cast<const T*>(dout), d_stride, scale, padding_idx,
-                                         static_cast<T*>(dweight), N, D));
+  const int64_t need = ghm_embed_rows_bwd_ws(N, V, D);
+  GHM_CHECK(ws_bytes >= need && (need == 0 || (ws && reinterpret_cast<uintptr_t>(ws) % 16 == 0)),
+            "workspace (too small, or not 16-byte aligned)");
+  TOK_DISPATCH(dtype, embed_bwd_any<T>(Ids{tokens, id_bits}, static_cast<const T*>(dout), d_stride, scale, padding_idx,
+                                       static_cast<T*>(dweight), N, V, static_cast<int>(D), static_cast<char*>(ws),
+                                       ghm_stream(stream)));
   return ghm_launch_status();
 }
