@@ -1197,25 +1197,22 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per;
   const int n = static_cast<int>(N - i0 < per ? N - i0 : per) * vecs;
   for (int t0 = threadIdx.x; t0 < n; t0 += 256 * U) {
+    int64_t v[U];
     float x[U][VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + 256 * u;
-      if (t >= n) break;
-      const int64_t v = ld_id(tok, i0 + t / vecs);
-      if (v >= 0 && v < V) {
-        load_cols<T, VE>(weight + v * w_stride, t % vecs * VE, D, x[u]);
-      } else {
+    for (int u = 0; u < U; ++u) v[u] = ld_id(tok, i0 + (t0 + 256 * u < n ? t0 + 256 * u : t0) / vecs);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) x[u][i] = __builtin_nanf("");
-      }
+    for (int u = 0; u < U; ++u) {  // every load is issued before the first is waited for; a bad token reads row 0
+      const int64_t row = v[u] >= 0 && v[u] < V ? v[u] : 0;
+      load_cols<T, VE>(weight + row * w_stride, (t0 + 256 * u < n ? t0 + 256 * u : t0) % vecs * VE, D, x[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int t = t0 + 256 * u;
       if (t >= n) break;
+      const float f = v[u] >= 0 && v[u] < V ? scale : __builtin_nanf("");
 #pragma unroll
-      for (int i = 0; i < VE; ++i) x[u][i] *= scale;
+      for (int i = 0; i < VE; ++i) x[u][i] *= f;
       store_cols<T, VE>(out + (i0 + t / vecs) * D, t % vecs * VE, D, x[u]);
     }
   }
@@ -1355,6 +1352,91 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
   }
 }
 
+// Up to SORT_ONE positions of a table of at most USED_ONE rows: all passes by one block,
+// key and position in one word of LDS between them.
+constexpr int POS_BITS = 14, SORT_ONE = 1 << POS_BITS, USED_ONE = (1 << (32 - POS_BITS)) - 1;
+template <int ROUNDS>
+__global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes, int bits, uint32_t* __restrict__ key_out,
+                                                   uint32_t* __restrict__ pos_out, uint32_t* __restrict__ used,
+                                                   int used_words) {
+  constexpr int W = 16;
+  __shared__ uint32_t word[1024 * ROUNDS], wbins[W][SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 64];
+  __shared__ uint16_t rank[1024 * ROUNDS];  // among the wave's equal digits
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i0 = w * 64 * ROUNDS + lane;
+  for (int j = threadIdx.x; j < used_words; j += 1024) used[j] = 0;
+#pragma unroll
+  for (int q = 0; q < ROUNDS; ++q) {
+    const int i = i0 + q * 64;
+    if (i < N) word[i] = sort_in(in, i) << POS_BITS | i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = POS_BITS + p * bits;
+    for (int d = lane; d < SORT_BINS; d += 64) wbins[w][d] = 0;
+    wave_fence();  // a wave ranks the words that it wrote, or that a barrier has passed
+    for (int i = i0; i - lane < N && i < i0 + 64 * ROUNDS; i += 64) {
+      const bool live = i < N;
+      const uint32_t d = live ? (word[i] >> shift) & (SORT_BINS - 1) : 0;
+      uint64_t same = __ballot(live);
+#pragma unroll
+      for (int bit = 0; bit < SORT_BITS; ++bit) {
+        const uint64_t m = __ballot((d >> bit) & 1);
+        same &= (d >> bit) & 1 ? m : ~m;
+      }
+      const uint64_t lower = same & ((uint64_t(1) << lane) - 1);
+      const uint32_t before = wbins[w][d];
+      if (live) rank[i] = static_cast<uint16_t>(before + __popcll(lower));
+      wave_fence();
+      if (live && lower == 0) wbins[w][d] = before + __popcll(same);
+      wave_fence();
+    }
+    __syncthreads();
+    if (threadIdx.x < SORT_BINS) {  // counts become starts: over the waves, then over the digits
+      const int d = threadIdx.x;
+      uint32_t all = 0;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const uint32_t c = wbins[j][d];
+        wbins[j][d] = all;
+        all += c;
+      }
+      uint32_t inc = all;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(inc, o, 64);
+        inc += lane >= o ? up : 0;
+      }
+      if (lane == 63) wsum[d >> 6] = inc;
+      base[d] = inc - all;
+    }
+    __syncthreads();
+    if (threadIdx.x < SORT_BINS)
+      for (int j = 0; j < static_cast<int>(threadIdx.x) >> 6; ++j) base[threadIdx.x] += wsum[j];
+    __syncthreads();
+    uint32_t x[ROUNDS], to[ROUNDS];
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q) {
+      const int i = i0 + q * 64;
+      x[q] = i < N ? word[i] : 0;
+      const uint32_t d = (x[q] >> shift) & (SORT_BINS - 1);
+      to[q] = i < N ? base[d] + wbins[w][d] + rank[i] : 0;
+      if (p == 0 && i < N && x[q] >> POS_BITS != in.none)
+        reinterpret_cast<uint8_t*>(used)[x[q] >> POS_BITS] = 1;  // cleared before the barriers
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q)
+      if (i0 + q * 64 < N) word[to[q]] = x[q];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int q = 0; q < ROUNDS; ++q) {
+    const int i = i0 + q * 64;
+    if (i >= N) break;
+    key_out[i] = word[i] >> POS_BITS;
+    pos_out[i] = word[i] & (SORT_ONE - 1);
+  }
+}
+
 // Chunk c of the sorted list, columns col .. col + VE - 1 per lane; `lpr` lanes per row,
 // 64 / lpr chunks per wave.  A token inside the chunk is finished here; one that goes on
 // from the chunk before leaves its sum in parts[c][0], one that begins here and goes on
@@ -1397,14 +1479,29 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
       store_cols<T, VE>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
     }
   };
+  // keys and positions of the next step are read ahead (16 bytes each: chunks are multiples
+  // of U, and the arrays are padded); entries past the end take row 0 and are not used
+  static_assert(U == 8, "two 16-byte reads per step");
+  u32x4 kn[2], pn[2];
+  const auto ahead = [&](int64_t i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      kn[h] = reinterpret_cast<const u32x4*>(key + i)[h];
+      pn[h] = reinterpret_cast<const u32x4*>(pos + i)[h];
+    }
+  };
+  ahead(lo);
   for (int64_t i = lo; i < hi; i += U) {
     uint32_t k[U];
     float x[U][VE];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      k[u] = i + u < hi ? key[i + u] : none;
-      if (k[u] != none) load_cols<T, VE>(dout + static_cast<int64_t>(pos[i + u]) * d_stride, col, D, x[u]);
+      k[u] = kn[u / 4][u % 4];
+      const int64_t row = i + u < hi ? pn[u / 4][u % 4] : 0;
+      load_cols<T, VE>(dout + row * d_stride, col, D, x[u]);
     }
+    if (k[0] == none) break;  // only tokens without a gradient follow
+    if (i + U < hi) ahead(i + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= hi) break;
@@ -1415,27 +1512,26 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc[e] = 0.f;
       }
-      if (cur != none) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += x[u][e];
-      }
+      for (int e = 0; e < VE; ++e) acc[e] += x[u][e];
     }
   }
+  if (cur == none) return;
   flush(hi < N && key[hi] == cur);
 }
 
 // A token that begins in chunk c and goes on: parts[c][1] + parts[c + 1][0] + ... in order,
-// a quarter of them per wave.
+// a quarter of them per wave, 4 columns per lane.
 template <typename T>
 __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ key, uint32_t none, float scale,
                                                     T* __restrict__ dw, int64_t N, int D, int chunk, int64_t chunks,
                                                     const float* __restrict__ parts) {
-  __shared__ float red[4][64];
+  __shared__ float red[4][4][64];
   const int64_t c = blockIdx.x, lo = c * chunk, hi = lo + chunk;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.y * 64 + lane;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.y * 256 + lane * 4;
   if (hi >= N) return;
-  const uint32_t k = key[hi];
-  if (k == none || key[hi - 1] != k || (lo > 0 && key[lo - 1] == k)) return;
+  const uint32_t k = key[hi], last = key[hi - 1], before = key[lo > 0 ? lo - 1 : 0];
+  if (k == none || last != k || (lo > 0 && before == k)) return;
   int64_t n = 1;  // chunks c .. c + n - 1 hold the token
   for (int64_t j = c + 1 + lane;; j += 64) {
     const uint64_t m = __ballot(j < chunks && key[j * chunk] == k);
@@ -1447,15 +1543,25 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
     break;
   }
   const int64_t q = (n + 3) / 4, a = w * q, b = a + q < n ? a + q : n;
-  float s = 0.f;
+  float s[4] = {};
   if (col < D) {
 #pragma unroll 8
-    for (int64_t j = a; j < b; ++j) s += parts[((c + j) * 2 + (j == 0 ? 1 : 0)) * D + col];
+    for (int64_t j = a; j < b; ++j) {
+      float x[4];
+      load_cols<float, 4>(parts + ((c + j) * 2 + (j == 0 ? 1 : 0)) * D, col, D, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += x[i];
+    }
   }
-  red[w][lane] = s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[w][i][lane] = s[i];
   __syncthreads();
-  if (w == 0 && col < D)
-    from_f(dw[static_cast<int64_t>(k) * D + col], (((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane]) * scale);
+  if (w != 0 || col >= D) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < D)
+      from_f(dw[static_cast<int64_t>(k) * D + col + i],
+             (((red[0][i][lane] + red[1][i][lane]) + red[2][i][lane]) + red[3][i][lane]) * scale);
 }
 
 // no token at all: every table row is 0
@@ -1777,6 +1883,7 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
 namespace {
 struct EmbedPlan {
   int W, passes, bits, chunk, slices, lpr;
+  bool one;
   int64_t tiles, chunks, used_words;
   int64_t key[2], pos[2], counts, used, parts, bytes;  // byte offsets in the workspace
 };
@@ -1787,13 +1894,14 @@ inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
   while (bits < 32 && (int64_t(1) << bits) <= V) ++bits;  // keys 0 .. V
   p.passes = (bits + SORT_BITS - 1) / SORT_BITS;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.W = N <= 65536 ? 4 : 16;
+  p.W = N <= 64 * 4 * SORT_ROUNDS * SORT_TILES ? 4 : 16;
+  p.one = N <= SORT_ONE && V <= USED_ONE;
   const int64_t tile = 64 * p.W * SORT_ROUNDS;
   p.tiles = (N + tile - 1) / tile;
   p.lpr = 1;
   while (p.lpr < 64 && p.lpr * ve < D) p.lpr *= 2;
   p.slices = static_cast<int>((D + p.lpr * ve - 1) / (p.lpr * ve));
-  const int64_t want = N * p.slices / (4096 * (64 / p.lpr));
+  const int64_t want = N * p.slices / (2048 * (64 / p.lpr));
   p.chunk = 16;
   while (p.chunk < 256 && p.chunk < want) p.chunk *= 2;
   p.chunks = (N + p.chunk - 1) / p.chunk;
@@ -1840,10 +1948,21 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
     return;
   }
   const EmbedPlan p = embed_plan(N, V, D, Vec<T>::N);
-  if (p.W == 4) launch_sort<4>(p, tok, pad, N, V, ws, s);
-  else launch_sort<16>(p, tok, pad, N, V, ws, s);
-  const uint32_t* key = reinterpret_cast<uint32_t*>(ws + p.key[(p.passes - 1) & 1]);
-  const uint32_t* pos = reinterpret_cast<uint32_t*>(ws + p.pos[(p.passes - 1) & 1]);
+  uint32_t* key = reinterpret_cast<uint32_t*>(ws + p.key[(p.passes - 1) & 1]);
+  uint32_t* pos = reinterpret_cast<uint32_t*>(ws + p.pos[(p.passes - 1) & 1]);
+  if (p.one) {
+    const SortIn in{tok, nullptr, nullptr, pad, static_cast<uint32_t>(V)};
+    uint32_t* flags = reinterpret_cast<uint32_t*>(ws + p.used);
+    const int n = static_cast<int>(N), words = static_cast<int>(p.used_words);
+    if (N <= 4096)
+      hipLaunchKernelGGL(k_sort_one<4>, dim3(1), dim3(1024), 0, s, in, n, p.passes, p.bits, key, pos, flags, words);
+    else
+      hipLaunchKernelGGL(k_sort_one<16>, dim3(1), dim3(1024), 0, s, in, n, p.passes, p.bits, key, pos, flags, words);
+  } else if (p.W == 4) {
+    launch_sort<4>(p, tok, pad, N, V, ws, s);
+  } else {
+    launch_sort<16>(p, tok, pad, N, V, ws, s);
+  }
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   const uint8_t* used = reinterpret_cast<uint8_t*>(ws + p.used);
   const int64_t sum_blocks = (p.chunks * p.slices * p.lpr + 255) / 256;
@@ -1857,7 +1976,7 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
                      static_cast<uint32_t>(V), dout, d_stride, scale, dw, N, D, p.chunk, p.chunks, p.slices, p.lpr,
                      sum_blocks, parts, used, V, static_cast<int>(rpb));
   if (p.chunks > 1)
-    hipLaunchKernelGGL(k_embed_join<T>, dim3(static_cast<unsigned>(p.chunks - 1), static_cast<unsigned>((D + 63) / 64)),
+    hipLaunchKernelGGL(k_embed_join<T>, dim3(static_cast<unsigned>(p.chunks - 1), static_cast<unsigned>((D + 255) / 256)),
                        dim3(256), 0, s, key, static_cast<uint32_t>(V), scale, dw, N, D, p.chunk, p.chunks, parts);
 }
 }  // namespace

@@ -78,16 +78,18 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# the handle of a device's current stream without a torch.cuda.Stream object around it
+# (2 us of a 15 us call, 9 us on autograd's thread)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device, name, *args):
     """Call an entry point on the device's current stream."""
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _native.call(name, *args, torch.cuda.current_stream().cuda_stream)
-    return _native.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _scratch(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            return _native.call(name, *args, _raw_stream(device.index))
+    return _native.call(name, *args, _raw_stream(device.index))
 
 
 def _check_logits(logits):
@@ -106,14 +108,13 @@ def _score(logits, targets, top_k, ignore_index, want_stats):
     z, n_inner, so, si = _rows(logits)
     rows = logits.numel() // V
     y, bits = (None, 64) if targets is None else _ids(targets, lead, dev, "targets")
-    f = torch.empty((4 if want_stats else 2, rows), dtype=torch.float32, device=dev)
-    logprob = None if y is None else f[0].view(lead)
-    entropy = f[1].view(lead)
-    stats = f[2:] if want_stats else None
+    logprob = None if y is None else torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
     top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=dev) if top_k else None
     top_id = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
     nws = _native.hip_lib().ghm_token_logprobs_ws(rows, V, top_k, code)
-    ws = _scratch(nws, dev)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     _call(dev, "ghm_token_logprobs", z.data_ptr(), code, n_inner, so, si, rows, V, _ptr(y), bits, ignore_index, top_k,
           _ptr(logprob), entropy.data_ptr(), _ptr(stats), _ptr(top_lp), _ptr(top_id), _ptr(ws), nws)
     return logprob, entropy, top_lp, top_id, stats
@@ -197,40 +198,41 @@ def _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, igno
 
 
 def _distill(logits, args, reduction, grad_scale=None):
-    """(loss, row_loss, stats, norm, dlogits or None) of ghm_distill."""
+    """(loss, stats, norm, dlogits or None) of ghm_distill: the statistics, the norm, the
+    row losses of a reduced loss and the workspace share one buffer."""
     dev, code, rows, V = logits.device, args[1], args[5], args[6]
-    f = torch.empty(2 + 5 * rows + (-rows) % 4 + 2, dtype=torch.float32, device=dev)
-    r4 = rows + (-rows) % 4  # loss and norm first, then the row losses; 16-byte aligned statistics last
-    loss, norm, row_loss, stats = f[0:1], f[1:2], f[4:4 + rows], f[4 + r4:]
     dz = None if grad_scale is None else torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    loss = torch.empty(logits.shape[:-1] if reduction == "none" else (), dtype=torch.float32, device=dev)
     nws = _native.hip_lib().ghm_distill_ws(rows, V, code)
-    ws = _scratch(nws, dev)
-    _call(dev, "ghm_distill", *args, _REDUCTION[reduction], loss.data_ptr(), row_loss.data_ptr(), stats.data_ptr(),
-          norm.data_ptr(), 1.0 if grad_scale is None else grad_scale, _ptr(dz), _ptr(ws), nws)
-    loss = row_loss.view(logits.shape[:-1]) if reduction == "none" else loss.view(())
-    return loss, stats, norm, dz
+    r4 = rows + (-rows) % 4
+    buf = torch.empty(4 * rows + 4 + r4 + nws // 4 + 4, dtype=torch.float32, device=dev)
+    at = buf.data_ptr()  # stats, norm, row losses, workspace; each at a multiple of 16 bytes
+    row_loss = loss.data_ptr() if reduction == "none" else at + 16 * (rows + 1)
+    _call(dev, "ghm_distill", *args, _REDUCTION[reduction], loss.data_ptr(), row_loss, at, at + 16 * rows,
+          1.0 if grad_scale is None else grad_scale, _ptr(dz), at + 16 * (rows + 1) + 4 * r4, nws)
+    return loss, buf, at + 16 * rows, dz
 
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_ids, top_logits, targets, temperature, alpha, ignore_index, reduction):
         args, _keep = _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index)
-        loss, stats, norm, _ = _distill(logits, args, reduction)
+        loss, buf, _, _ = _distill(logits, args, reduction)
         ctx.opts = (temperature, alpha, ignore_index)
         ctx.reduction = reduction
-        ctx.save_for_backward(logits, top_ids, top_logits, targets, stats, norm)
+        ctx.save_for_backward(logits, top_ids, top_logits, targets, buf)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, top_ids, top_logits, targets, stats, norm = ctx.saved_tensors
+        logits, top_ids, top_logits, targets, buf = ctx.saved_tensors
         args, _keep = _distill_args(logits, top_ids, top_logits, targets, *ctx.opts)
         g = g.contiguous()
         dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _call(logits.device, "ghm_distill_bwd", *args, stats.data_ptr(),
-              norm.data_ptr() if ctx.reduction == "mean" else None, g.data_ptr(), int(ctx.reduction == "none"),
-              dz.data_ptr())
+        at = buf.data_ptr()
+        _call(logits.device, "ghm_distill_bwd", *args, at, at + 16 * args[5] if ctx.reduction == "mean" else None,
+              g.data_ptr(), int(ctx.reduction == "none"), dz.data_ptr())
         return (dz, *[None] * 7)
 
 
@@ -322,7 +324,7 @@ class _EmbedFn(torch.autograd.Function):
             g, si = g.contiguous(), D
         dw = torch.empty(V, D, dtype=g.dtype, device=g.device)
         nws = _native.hip_lib().ghm_embed_rows_bwd_ws(N, V, D)
-        ws = _scratch(nws, g.device)
+        ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws else None
         _call(g.device, "ghm_embed_rows_bwd", tok.data_ptr(), bits, g.data_ptr(), _DTYPE[g.dtype], si, ctx.scale,
               ctx.padding_idx, dw.data_ptr(), N, V, D, _ptr(ws), nws)
         return None, dw, None, None
