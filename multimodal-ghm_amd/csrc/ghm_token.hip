@@ -45,6 +45,21 @@ __device__ __forceinline__ int64_t ld_id(const Ids& t, int64_t i) {
   return static_cast<const uint8_t*>(t.p)[i];
 }
 
+// several at once: no load waits for another's branch
+template <int U, typename F>
+__device__ __forceinline__ void ld_ids(const Ids& t, int64_t (&id)[U], F at) {
+  if (t.bits == 64) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = static_cast<const int64_t*>(t.p)[at(u)];
+  } else if (t.bits == 32) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = static_cast<const int32_t*>(t.p)[at(u)];
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = static_cast<const uint8_t*>(t.p)[at(u)];
+  }
+}
+
 // Order of the alternatives: value descending (NaN above all, -0 equal to +0),
 // then id ascending, as one unsigned 64-bit key per entry.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -70,18 +85,18 @@ struct Vec<float> {
   static constexpr int N = 4;
   using raw = u32x4_a4;
 };
+template <typename T, int N>
+__device__ __forceinline__ void unpack(u32x4 v, float (&x)[N]) {
+  static_assert(N == Vec<T>::N, "16 bytes");
+  T e[N];
+  __builtin_memcpy(e, &v, 16);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = to_f(e[i]);
+}
 template <int N, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
-  if constexpr (N == 1) {
-    x[0] = to_f(*p);
-  } else {
-    static_assert(N == Vec<T>::N, "one value or 16 bytes");
-    const u32x4 v = *reinterpret_cast<const typename Vec<T>::raw*>(p);
-    T e[N];
-    __builtin_memcpy(e, &v, 16);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f(e[i]);
-  }
+  if constexpr (N == 1) x[0] = to_f(*p);
+  else unpack<T>(*reinterpret_cast<const typename Vec<T>::raw*>(p), x);
 }
 template <int N, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
@@ -203,8 +218,10 @@ __device__ __forceinline__ Sums group_join(Sums a, float* slots, int w, float c1
 // maximum: the waves hold k vectors at or above it; (b) a wave's own k-th vector after a
 // prune, strictly, for its later (higher) indices.  That is one comparison per vector, and
 // a few hundred vectors of a row are noted; at the end they are ranked by counting, and
-// the values of the k best ones, read again, are ranked the same way.
-constexpr int TOP_CAP = 256;  // vectors noted per wave: 64 kept by a prune, 64 per step
+// the values of the k best ones, read again, are ranked the same way.  The maxima skip NaN:
+// a range whose sum is NaN (a NaN or +inf in it) is searched value by value instead.
+constexpr int TOP_CAP = 384;  // vectors noted per wave: pruned where a batch might not fit
+constexpr int TOP_BATCH = 256;  // vectors of a wave's batch, at most
 
 // at least r lanes hold u >= the result (its upper 16 bits are searched: a lower bound
 // of the r-th largest); 0: fewer
@@ -229,26 +246,19 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
-// keep the k largest of a wave's n candidates, in descending order
-__device__ __forceinline__ void top_prune(uint64_t* cand, int n, int k, int lane) {
-  constexpr int M = TOP_CAP / 64;
-  uint64_t mine[M];
-  int rank[M];
+// keep the k largest of a wave's n candidates, in descending order (spare: 64 words)
+__device__ __forceinline__ void top_prune(uint64_t* cand, uint64_t* spare, int n, int k, int lane) {
   wave_fence();
-#pragma unroll
-  for (int j = 0; j < M; ++j) {
-    mine[j] = lane + 64 * j < n ? cand[lane + 64 * j] : 0;
-    rank[j] = 0;
-  }
-  for (int i = 0; i < n; ++i) {
-    const uint64_t c = cand[i];
-#pragma unroll
-    for (int j = 0; j < M; ++j) rank[j] += c > mine[j];
+#pragma unroll 1
+  for (int j = lane; j < n; j += 64) {
+    const uint64_t mine = cand[j];
+    int rank = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) rank += cand[i] > mine;
+    if (rank < k) spare[rank] = mine;
   }
   wave_fence();
-#pragma unroll
-  for (int j = 0; j < M; ++j)
-    if (lane + 64 * j < n && rank[j] < k) cand[rank[j]] = mine[j];
+  if (lane < k) cand[lane] = spare[lane];
   wave_fence();
 }
 
@@ -264,32 +274,39 @@ struct TopState {
   uint32_t bound = 0;  // the group's bound (a) as order bits
 };
 
-// A row's values lo .. hi - 1: batches of U vectors of N values per lane; the values
-// after the last whole vector are one more vector, of lane 0 of wave 0.  The vectors of a
-// wave come in ascending order.  TOP: notes vectors for the k largest values.
+// A row's values lo .. hi - 1 (of at least N in the row up to hi): batches of U vectors of N
+// values per lane; the values after the last whole vector are one more vector, read as the
+// range's last N values with those that the vector before holds masked.  The vectors of
+// a wave come in ascending order.  TOP: notes vectors for the k largest values.
 template <typename T, int N, int U, int W, int SECOND, bool TOP>
 __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, float c2, int w, int lane, int k,
                                          TopLds<N, W>* lds, TopState& top) {
   Sums a;
   float thr = __builtin_nanf("");
-  const int nv = (hi - lo) / N, tail = (hi - lo) - nv * N;
+  const int tail = (hi - lo) % N, nv = (hi - lo) / N + (tail ? 1 : 0);
   const int r = TOP ? (k + W - 1) / W : 0;
   constexpr int STEP = W * 64 * U;
-  const int full = (nv + STEP - 1) / STEP, nb = full + (tail ? 1 : 0);
+  const int nb = (nv + STEP - 1) / STEP;
   uint64_t* cand = TOP ? lds->cand + w * TOP_CAP : nullptr;
   for (int b = 0; b < nb; ++b) {
     float x[U][N], vm[U];
-    const int v0 = b < full ? b * STEP + w * 64 + lane : nv + w * 64 + lane;
+    const int v0 = b * STEP + w * 64 + lane;
+    if (b < nb - 1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < U; ++u) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
+    } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u][i] = NEG_INF;
-      if (v0 + u * W * 64 < nv) load_vec<N>(z + lo + (v0 + u * W * 64) * N, x[u]);
-    }
-    if (N > 1 && b == full && v0 == nv) {
+      for (int u = 0; u < U; ++u) {  // lanes past the end read the last vector again
+        const int v = v0 + u * W * 64, at = v < nv ? v * N : (nv - 1) * N;
+        load_vec<N>(z + (lo + at + N <= hi ? lo + at : hi - N), x[u]);
+      }
 #pragma unroll
-      for (int i = 0; i < N - 1; ++i)
-        if (i < tail) x[0][i] = to_f(z[lo + nv * N + i]);
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * W * 64;
+        const int skip = v >= nv ? N : v == nv - 1 && tail ? N - tail : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[u][i] = i < skip ? NEG_INF : x[u][i];
+      }
     }
     float bm = -FLT_MAX;
 #pragma unroll
@@ -317,26 +334,17 @@ __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, f
         }
         thr = fmaxf(thr, below(top.bound));  // fmaxf takes the other of a NaN
       }
-      const bool nan = a.s != a.s;  // a NaN or +inf was seen; the maxima skip NaN
-      if (__ballot(nan || !(bm <= thr)) == 0) continue;
-      if (__ballot(nan)) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < N; ++i) vm[u] = x[u][i] != x[u][i] ? x[u][i] : vm[u];
+      if (__ballot(!(bm <= thr)) == 0) continue;
+      static_assert(64 * U <= TOP_BATCH, "a batch fits beside what a prune leaves");
+      if (top.cnt > TOP_CAP - TOP_BATCH) {
+        top_prune(cand, lds->merged + w * 64, top.cnt, k, lane);
+        top.cnt = k;
+        thr = fmaxf(thr, key_value(cand[k - 1]));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int v = v0 + u * W * 64;
-        const bool valid = v < nv + (tail && b == full);
-        uint64_t mask = __ballot(valid && !(vm[u] <= thr));
-        if (mask == 0) continue;
-        if (top.cnt + __popcll(mask) > TOP_CAP) {
-          top_prune(cand, top.cnt, k, lane);
-          top.cnt = k;  // of at least TOP_CAP - 63 > k
-          thr = fmaxf(thr, key_value(cand[k - 1]));
-          mask = __ballot(valid && !(vm[u] <= thr));
-        }
+        const uint64_t mask = __ballot(v < nv && !(vm[u] <= thr));
         if ((mask >> lane) & 1) cand[top.cnt + __popcll(mask & ((uint64_t(1) << lane) - 1))] = top_key(vm[u], v);
         top.cnt += __popcll(mask);
       }
@@ -353,7 +361,7 @@ __device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N,
                                            int lane, F emit) {
   uint64_t* cand = lds->cand + w * TOP_CAP;
   if (top.cnt > 64) {
-    top_prune(cand, top.cnt, k, lane);
+    top_prune(cand, lds->merged + w * 64, top.cnt, k, lane);
     top.cnt = k;
   }
   group_sync<W>();  // every wave's last bound is there
@@ -425,6 +433,34 @@ __device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N,
 // H = log s - sum e^(z - m) (z - m) / s.  A value of -inf has probability 0 and
 // adds nothing; a row without a finite maximum has no distribution (NaN).
 // ---------------------------------------------------------------------------
+// The same by k searches of the whole range, for one that holds NaN or +inf.
+template <typename T, int N, int W, typename F>
+__device__ __forceinline__ void top_search(const T* z, int lo, int hi, TopLds<N, W>* lds, int k, int w, int lane,
+                                           F emit) {
+  uint64_t last = ~uint64_t(0);
+  for (int j = 0; j < k; ++j) {
+    uint64_t best = 0;
+    for (int v = lo + w * 64 + lane; v < hi; v += W * 64) {
+      const uint64_t key = top_key(to_f(z[v]), v);
+      best = key < last && key > best ? key : best;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint64_t other = __shfl_xor(best, o, 64);
+      best = other > best ? other : best;
+    }
+    if constexpr (W > 1) {
+      if (lane == 0) lds->merged[w] = best;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) best = lds->merged[i] > best ? lds->merged[i] : best;
+      __syncthreads();
+    }
+    if (w == 0 && lane == 0) emit(j, best);
+    last = best;
+  }
+}
+
 struct ScoreOut {
   float *logprob, *entropy;
   float2* stats;
@@ -494,10 +530,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
   }
   if constexpr (TOP) {
     const float ls = logf(a.s);
-    top_finish<T>(z, lo, hi, lds, top, out.top_k, w, lane, [&](int j, uint64_t key) {
+    const auto emit = [&](int j, uint64_t key) {
       if (part_sums) part_keys[item * out.top_k + j] = key;
       else score_top(out, r, j, key, a.m, ls);
-    });
+    };
+    if (a.s == a.s) top_finish<T>(z, lo, hi, lds, top, out.top_k, w, lane, emit);
+    else top_search<T>(z, lo, hi, lds, out.top_k, w, lane, emit);
   }
 }
 
@@ -596,6 +634,9 @@ __global__ __launch_bounds__(256) void k_score_short(Rows rows, int64_t n_rows, 
 struct Split {
   int parts, len;
 };
+inline bool one_wave(int64_t rows, int64_t V, int N) {
+  return V <= 256 * N || (V <= 1536 * N && rows >= 1024);
+}
 inline Split row_split(int64_t rows, int64_t V) {
   const int64_t most = V / 4096;
   int64_t p = rows > 0 && rows < 512 ? (512 + rows - 1) / rows : 1;
@@ -920,43 +961,63 @@ __device__ __forceinline__ float distill_row_loss(const T* z, int V, const Teach
   return loss;
 }
 
-// The gradient of values lo .. hi - 1 of a row: the two softmaxes everywhere first, then
-// the teacher's and the target's entries again (a repeated id writes its sum each time).
-template <typename T, int N, int U, int W>
-__device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int hi, const Teacher& tc, const Mix& mix,
-                                                 const TeacherRow& tr, const TeacherLds<W>& lds, float m, float l1,
-                                                 float l2, int64_t y, float scale, int w, int lane) {
-  const float A = tr.some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : 0.f;
-  const float B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
-  const float k1 = -l1 * LOG2E, k2 = -l2 * LOG2E, e2 = mix.it * LOG2E;
-  // one exponential where the softmaxes are the same one, or only one of them counts
-  const bool one = !mix.two;
-  const float c = A != 0.f || !mix.hard ? e2 : LOG2E, k = A != 0.f || !mix.hard ? k2 : k1, AB = A + B;
-  const bool none = A == 0.f && B == 0.f;
-  if (none && scale == scale) {
-    zero_row<T, N, W>(d, lo, hi, w, lane);
-    return;
+// The gradient of a row: the two softmaxes everywhere, then the teacher's and the target's
+// entries again.
+struct DistillGrad {
+  float A, B, m, e, k, k1, AB;  // e, k: the teacher's exponent factor and offset, or the only one's
+  bool two, none;
+  __device__ __forceinline__ float one(float x) const { return AB * __builtin_amdgcn_exp2f(__builtin_fmaf(x - m, e, k)); }
+  __device__ __forceinline__ float both(float x) const {
+    const float d = x - m;
+    return __builtin_fmaf(A, __builtin_amdgcn_exp2f(__builtin_fmaf(d, e, k)),
+                          B * __builtin_amdgcn_exp2f(__builtin_fmaf(d, LOG2E, k1)));
   }
-  const auto soft1 = [=](float x) { return AB * __builtin_amdgcn_exp2f(__builtin_fmaf(x - m, c, k)); };
-  const auto soft2 = [=](float x) {
-    const float dx = x - m;
-    return __builtin_fmaf(A, __builtin_amdgcn_exp2f(__builtin_fmaf(dx, e2, k2)),
-                          B * __builtin_amdgcn_exp2f(__builtin_fmaf(dx, LOG2E, k1)));
-  };
-  if (one) map_row<T, N, U, W>(z, d, lo, hi, w, lane, soft1);
-  else map_row<T, N, U, W>(z, d, lo, hi, w, lane, soft2);
-  group_sync<W>();
+};
+__device__ __forceinline__ DistillGrad distill_grad(const Mix& mix, bool some, float m, float l1, float l2, float scale) {
+  DistillGrad g;
+  g.A = some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : 0.f;
+  g.B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
+  g.AB = g.A + g.B;
+  g.m = m;
+  g.k1 = -l1 * LOG2E;
+  // one exponential where the softmaxes are the same one, or only one of them counts
+  const bool hard_only = !mix.two && g.A == 0.f && mix.hard;
+  g.e = hard_only ? LOG2E : mix.c2;
+  g.k = hard_only ? g.k1 : -l2 * LOG2E;
+  g.two = mix.two;
+  g.none = g.A == 0.f && g.B == 0.f && scale == scale;
+  return g;
+}
+// the entries among values lo .. hi - 1, after the group's stores (a repeated id writes its
+// sum each time)
+template <typename T, int W>
+__device__ __forceinline__ void distill_entries(const T* z, T* d, int lo, int hi, const Teacher& tc, const Mix& mix,
+                                                const DistillGrad& g, const TeacherLds<W>& lds, int64_t y, int w,
+                                                int lane) {
   const auto entry = [&](int id) {
     const float x = to_f(z[id]);
-    float g = one ? soft1(x) : soft2(x), q = 0.f;
+    float v = g.two ? g.both(x) : g.one(x), q = 0.f;
     for (int j = 0; j < tc.k; ++j) q += lds.id[j] == id ? lds.q[j] : 0.f;
-    g -= A * q;
-    if (id == y) g -= B;
-    from_f(d[id], g);
+    v -= g.A * q;
+    if (id == y) v -= g.B;
+    from_f(d[id], v);
   };
   for (int j = w * 64 + lane; j < tc.k; j += W * 64)
     if (lds.id[j] >= lo && lds.id[j] < hi) entry(lds.id[j]);
   if (mix.hard && y >= lo && y < hi && w == 0 && lane == 0) entry(static_cast<int>(y));
+}
+template <typename T, int N, int U, int W>
+__device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int hi, const Teacher& tc, const Mix& mix,
+                                                 const DistillGrad& g, const TeacherLds<W>& lds, int64_t y, int w,
+                                                 int lane) {
+  if (g.none) {
+    zero_row<T, N, W>(d, lo, hi, w, lane);
+    return;
+  }
+  if (g.two) map_row<T, N, U, W>(z, d, lo, hi, w, lane, [=](float x) { return g.both(x); });
+  else map_row<T, N, U, W>(z, d, lo, hi, w, lane, [=](float x) { return g.one(x); });
+  group_sync<W>();
+  distill_entries<T, W>(z, d, lo, hi, tc, mix, g, lds, y, w, lane);
 }
 
 // Sums of a row, its loss, and its gradient if dz is there, by a group of W waves.
@@ -998,8 +1059,104 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
     row_stats[r] = make_float4(a.m, l1, l2, 1.f);
   }
   if (d)
-    distill_row_grad<T, N, U, W>(z, d, 0, V, tc, mix, tr, lds, a.m, l1, l2, y,
-                                 bad ? __builtin_nanf("") : upstream(up, r, lane), w, lane);
+    distill_row_grad<T, N, U, W>(z, d, 0, V, tc, mix,
+                                 distill_grad(mix, tr.some, a.m, l1, l2, bad ? __builtin_nanf("") : upstream(up, r, lane)),
+                                 lds, y, w, lane);
+}
+
+// Packed values stay packed across this point: without it the compiler keeps the unpacked
+// floats from one pass to the next, twice the registers of 16-bit values.
+template <int R>
+__device__ __forceinline__ void hold(u32x4 (&raw)[R]) {
+#pragma unroll
+  for (int u = 0; u < R; ++u) asm volatile("" : "+v"(raw[u]));
+}
+
+// The same with the row held in registers between the sums and the gradient (R vectors per
+// lane, R * 64 * W * N values at most): the logits are read once.
+template <typename T, int R, int W, bool TWO>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_distill_step(Rows rows, int64_t n_rows, int V, Teacher tc,
+                                                                        Ids targets, int64_t ignore, Mix mix,
+                                                                        Upstream up, float* __restrict__ row_loss,
+                                                                        float4* __restrict__ row_stats,
+                                                                        T* __restrict__ dz) {
+  constexpr int G = W == 1 ? 4 : 1, N = Vec<T>::N, SECOND = TWO ? SECOND_EXP : SECOND_NONE;
+  __shared__ float slots[3 * W];
+  __shared__ TeacherLds<W> teach[G];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  if (r >= n_rows) return;
+  T* d = dz + r * V;
+  if (!row_counts(tc, targets, ignore, r, lane)) {
+    if (w == 0 && lane == 0) {
+      row_loss[r] = 0.f;
+      row_stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    zero_row<T, N, W>(d, 0, V, w, lane);
+    return;
+  }
+  const T* z = row_ptr<T>(rows, r);
+  const int64_t y = targets.p ? ld_id(targets, r) : -1;
+  // vectors as in scan_row: the last one of a row that does not divide is its last N values
+  const int tail = V % N, nv = V / N + (tail ? 1 : 0), v0 = w * 64 + lane;
+  u32x4 raw[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int v = v0 + u * W * 64, at = v < nv ? v * N : V - N;
+    raw[u] = *reinterpret_cast<const typename Vec<T>::raw*>(z + (at + N <= V ? at : V - N));
+  }
+  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
+  Sums a;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {  // values seen twice do not change a maximum
+    float x[N];
+    unpack<T>(raw[u], x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.m = fmaxf(a.m, x[i]);
+  }
+  a.m = group_max<W>(a.m, slots, w);
+  hold(raw);
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int v = v0 + u * W * 64;
+    if (v - lane >= nv) break;
+    float x[N];
+    unpack<T>(raw[u], x);
+    if (v - lane + 64 >= nv) {  // the wave's last vectors
+      const int skip = v >= nv ? N : v == nv - 1 && tail ? N - tail : 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = i < skip ? NEG_INF : x[i];
+    }
+    fold<SECOND>(a, x, mix.c1, mix.c2);
+  }
+  a.s = group_sum<W>(a.s, slots + W, w);
+  if constexpr (TWO) a.t = group_sum<W>(a.t, slots + 2 * W, w);
+  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  const float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
+  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  if (w == 0 && lane == 0) {
+    row_loss[r] = bad ? __builtin_nanf("") : loss;
+    row_stats[r] = make_float4(a.m, l1, l2, 1.f);
+  }
+  const DistillGrad g = distill_grad(mix, tr.some, a.m, l1, l2, bad ? __builtin_nanf("") : upstream(up, r, lane));
+  if (g.none) {
+    zero_row<T, N, W>(d, 0, V, w, lane);
+    return;
+  }
+  hold(raw);
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int v = v0 + u * W * 64;
+    if (v >= nv) break;
+    float x[N];
+    unpack<T>(raw[u], x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = TWO ? g.both(x[i]) : g.one(x[i]);
+    store_vec<N>(d + (v * N + N <= V ? v * N : V - N), x);
+  }
+  group_sync<W>();
+  distill_entries<T, W>(z, d, 0, V, tc, mix, g, lds, y, w, lane);
 }
 
 // long rows, few of them: the sums of one part of a row ...
@@ -1073,8 +1230,9 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
   TeacherLds<W>& lds = teach[wave / W];
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
   const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
-  distill_row_grad<T, N, U, W>(row_ptr<T>(rows, r), d, lo, hi, tc, mix, tr, lds, st.x, st.y, st.z, y,
-                               bad ? __builtin_nanf("") : upstream(up, r, lane), w, lane);
+  distill_row_grad<T, N, U, W>(
+      row_ptr<T>(rows, r), d, lo, hi, tc, mix,
+      distill_grad(mix, tr.some, st.x, st.y, st.z, bad ? __builtin_nanf("") : upstream(up, r, lane)), lds, y, w, lane);
 }
 
 // Rows of at most SHORT_V values, one lane per row: loss, statistics and gradient, each
@@ -1167,10 +1325,16 @@ __global__ __launch_bounds__(256) void k_distill_short(Rows rows, int64_t n_rows
 // ---------------------------------------------------------------------------
 // Scaled embedding: out_i = scale W[tok_i].
 // ---------------------------------------------------------------------------
-// up to VE values of a row from column c on (fewer at its end; the rest 0)
+// Rows of D values are taken in vectors of VE; the last one of a row that does not divide is
+// its last VE values, shared with the vector before (both hold the same results).  Rows
+// shorter than a vector go value by value.
+template <int VE>
+__device__ __forceinline__ int edge_col(int c, int D) {
+  return c + VE <= D || D < VE ? c : D - VE;
+}
 template <typename T, int VE>
 __device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&x)[VE]) {
-  if (c + VE <= D) {
+  if (D >= VE) {
     load_vec<VE>(row + c, x);
   } else {
 #pragma unroll
@@ -1179,7 +1343,7 @@ __device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&x)
 }
 template <typename T, int VE>
 __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&x)[VE]) {
-  if (c + VE <= D) {
+  if (D >= VE) {
     store_vec<VE>(row + c, x);
   } else {
 #pragma unroll
@@ -1199,12 +1363,12 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
   for (int t0 = threadIdx.x; t0 < n; t0 += 256 * U) {
     int64_t v[U];
     float x[U][VE];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld_id(tok, i0 + (t0 + 256 * u < n ? t0 + 256 * u : t0) / vecs);
+    ld_ids<U>(tok, v, [&](int u) { return i0 + (t0 + 256 * u < n ? t0 + 256 * u : t0) / vecs; });
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // every load is issued before the first is waited for; a bad token reads row 0
       const int64_t row = v[u] >= 0 && v[u] < V ? v[u] : 0;
-      load_cols<T, VE>(weight + row * w_stride, (t0 + 256 * u < n ? t0 + 256 * u : t0) % vecs * VE, D, x[u]);
+      load_cols<T, VE>(weight + row * w_stride, edge_col<VE>((t0 + 256 * u < n ? t0 + 256 * u : t0) % vecs * VE, D), D,
+                       x[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1213,7 +1377,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
       const float f = v[u] >= 0 && v[u] < V ? scale : __builtin_nanf("");
 #pragma unroll
       for (int i = 0; i < VE; ++i) x[u][i] *= f;
-      store_cols<T, VE>(out + (i0 + t / vecs) * D, t % vecs * VE, D, x[u]);
+      store_cols<T, VE>(out + (i0 + t / vecs) * D, edge_col<VE>(t % vecs * VE, D), D, x[u]);
     }
   }
 }
@@ -1227,19 +1391,26 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_ROUNDS = 8;
 constexpr int SORT_TILES = 128;  // up to this many tiles a block sums their counts itself
 
-// the sorted key of position i: its token; `none` for a token that gets no gradient
-__device__ __forceinline__ uint32_t sort_key(const Ids& tok, int64_t i, int64_t pad, uint32_t none) {
-  const int64_t v = ld_id(tok, i);
-  return v >= 0 && v < none && v != pad ? static_cast<uint32_t>(v) : none;
-}
+// The sorted key of a position is its token, or `none` for a token that gets no gradient.
 struct SortIn {  // the first pass reads tokens, later ones the previous pass's keys and positions
   Ids tok;
   const uint32_t *key, *pos;
   int64_t pad;
   uint32_t none;
 };
-__device__ __forceinline__ uint32_t sort_in(const SortIn& in, int64_t i) {
-  return in.key ? in.key[i] : sort_key(in.tok, i, in.pad, in.none);
+// keys of positions i, i + step, ... (the last one's again past the end: no load waits for a branch)
+template <int R>
+__device__ __forceinline__ void sort_in(const SortIn& in, int64_t i, int64_t step, int64_t N, uint32_t (&key)[R]) {
+  const auto at = [&](int q) { return i + q * step < N ? i + q * step : N - 1; };
+  if (in.key) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) key[q] = in.key[at(q)];
+  } else {
+    int64_t v[R];
+    ld_ids<R>(in.tok, v, at);
+#pragma unroll
+    for (int q = 0; q < R; ++q) key[q] = v[q] >= 0 && v[q] < in.none && v[q] != in.pad ? static_cast<uint32_t>(v[q]) : in.none;
+  }
 }
 
 // counts[tile][digit]; the first pass also clears the table of rows that have a token
@@ -1254,12 +1425,12 @@ __global__ __launch_bounds__(64 * W) void k_sort_count(SortIn in, int64_t N, int
          j += static_cast<int64_t>(gridDim.x) * 64 * W)
       used[j] = 0;
   __syncthreads();
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * TILE;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * TILE + threadIdx.x;
+  uint32_t key[SORT_ROUNDS];
+  sort_in<SORT_ROUNDS>(in, i0, 64 * W, N, key);
 #pragma unroll
-  for (int q = 0; q < SORT_ROUNDS; ++q) {
-    const int64_t i = i0 + q * 64 * W + threadIdx.x;
-    if (i < N) atomicAdd(&bins[(sort_in(in, i) >> shift) & (SORT_BINS - 1)], 1u);
-  }
+  for (int q = 0; q < SORT_ROUNDS; ++q)
+    if (i0 + q * 64 * W < N) atomicAdd(&bins[(key[q] >> shift) & (SORT_BINS - 1)], 1u);
   __syncthreads();
   for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d] = bins[d];
 }
@@ -1317,11 +1488,11 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
   }
   const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * W + w) * 64 * SORT_ROUNDS + lane;
   uint32_t key[SORT_ROUNDS], at[SORT_ROUNDS], pos[SORT_ROUNDS];
+  sort_in<SORT_ROUNDS>(in, i0, 64, N, key);
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
     const int64_t i = i0 + q * 64;
-    key[q] = i < N ? sort_in(in, i) : 0;
-    pos[q] = i < N && in.pos ? in.pos[i] : static_cast<uint32_t>(i);
+    pos[q] = in.pos ? in.pos[i < N ? i : N - 1] : static_cast<uint32_t>(i);
   }
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
@@ -1363,11 +1534,15 @@ __global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes,
   __shared__ uint32_t word[1024 * ROUNDS], wbins[W][SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 64];
   __shared__ uint16_t rank[1024 * ROUNDS];  // among the wave's equal digits
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i0 = w * 64 * ROUNDS + lane;
-  for (int j = threadIdx.x; j < used_words; j += 1024) used[j] = 0;
+  {
+    uint32_t key[ROUNDS];
+    sort_in<ROUNDS>(in, i0, 64, N, key);
+    for (int j = threadIdx.x; j < used_words; j += 1024) used[j] = 0;
 #pragma unroll
-  for (int q = 0; q < ROUNDS; ++q) {
-    const int i = i0 + q * 64;
-    if (i < N) word[i] = sort_in(in, i) << POS_BITS | i;
+    for (int q = 0; q < ROUNDS; ++q) {
+      const int i = i0 + q * 64;
+      if (i < N) word[i] = key[q] << POS_BITS | i;
+    }
   }
   for (int p = 0; p < passes; ++p) {
     const int shift = POS_BITS + p * bits;
@@ -1455,13 +1630,15 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
     const float zero[VE] = {};
     for (int64_t v = v0 + (threadIdx.x >> 6); v < v1; v += 4)
       if (!used[v])
-        for (int c = (threadIdx.x & 63) * VE; c < D; c += 64 * VE) store_cols<T, VE>(dw + v * D, c, D, zero);
+        for (int c = (threadIdx.x & 63) * VE; c < D; c += 64 * VE)
+          store_cols<T, VE>(dw + v * D, edge_col<VE>(c, D), D, zero);
     return;
   }
   const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / lpr;
   const int64_t c = group / slices;
-  const int col = (static_cast<int>(group % slices) * lpr + threadIdx.x % lpr) * VE;
-  if (c >= chunks || col >= D) return;
+  const int col0 = (static_cast<int>(group % slices) * lpr + threadIdx.x % lpr) * VE;
+  if (c >= chunks || col0 >= D) return;
+  const int col = edge_col<VE>(col0, D);
   const int64_t lo = c * chunk, hi = lo + chunk < N ? lo + chunk : N;
   uint32_t cur = key[lo];
   bool left = lo > 0 && key[lo - 1] == cur;
@@ -1469,10 +1646,18 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
   const auto flush = [&](bool right) {
     if (cur == none) return;
     if (left || right) {
-      float* o = parts + (c * 2 + (left ? 0 : 1)) * D;
+      float* o = parts + (c * 2 + (left ? 0 : 1)) * D + col;
+      if (D >= VE) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i)
-        if (col + i < D) o[col + i] = acc[i];
+        for (int h = 0; h < VE / 4; ++h) {
+          const float q[4] = {acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
+          store_vec<4>(o + 4 * h, q);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          if (col + i < D) o[i] = acc[i];
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < VE; ++i) acc[i] *= scale;
@@ -1528,7 +1713,8 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
                                                     const float* __restrict__ parts) {
   __shared__ float red[4][4][64];
   const int64_t c = blockIdx.x, lo = c * chunk, hi = lo + chunk;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.y * 256 + lane * 4;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col0 = blockIdx.y * 256 + lane * 4;
+  const int col = edge_col<4>(col0, D);
   if (hi >= N) return;
   const uint32_t k = key[hi], last = key[hi - 1], before = key[lo > 0 ? lo - 1 : 0];
   if (k == none || last != k || (lo > 0 && before == k)) return;
@@ -1544,7 +1730,7 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
   }
   const int64_t q = (n + 3) / 4, a = w * q, b = a + q < n ? a + q : n;
   float s[4] = {};
-  if (col < D) {
+  if (col0 < D) {
 #pragma unroll 8
     for (int64_t j = a; j < b; ++j) {
       float x[4];
@@ -1556,7 +1742,7 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
 #pragma unroll
   for (int i = 0; i < 4; ++i) red[w][i][lane] = s[i];
   __syncthreads();
-  if (w != 0 || col >= D) return;
+  if (w != 0 || col0 >= D) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (col + i < D)
@@ -1620,10 +1806,18 @@ void score_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore,
     const dim3 g(static_cast<unsigned>((rows + 255) / 256));
     if (V <= 12) hipLaunchKernelGGL((k_score_short<T, 12>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
     else hipLaunchKernelGGL((k_score_short<T, SHORT_V>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
-  } else if (V <= 512) {
-    launch_score<T, 1, 8, 1>(m, rows, V, t, ignore, o, p, ws, s);
-  } else if (V <= 2048) {
+  } else if (V <= 64) {
+    launch_score<T, 1, 1, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (V <= 256) {
+    launch_score<T, 1, 4, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (V <= 64 * N) {
+    launch_score<T, N, 1, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (V <= 128 * N) {
+    launch_score<T, N, 2, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (one_wave(rows, V, N)) {
     launch_score<T, N, 4, 1>(m, rows, V, t, ignore, o, p, ws, s);
+  } else if (o.top_k || V < 4096 * N) {
+    launch_score<T, N, 4, 4>(m, rows, V, t, ignore, o, p, ws, s);
   } else {
     launch_score<T, N, 4, 8>(m, rows, V, t, ignore, o, p, ws, s);
   }
@@ -1668,9 +1862,9 @@ void score_bwd_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ign
     const dim3 gr(static_cast<unsigned>((rows + 255) / 256));
     if (V <= 12) hipLaunchKernelGGL((k_score_bwd_short<T, 12>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
     else hipLaunchKernelGGL((k_score_bwd_short<T, SHORT_V>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
-  } else if (V <= 512) {
-    launch_score_bwd<T, 1, 8, 1>(m, rows, V, t, ignore, g, p, dz, s);
-  } else if (V <= 2048) {
+  } else if (V <= 256) {
+    launch_score_bwd<T, 1, 4, 1>(m, rows, V, t, ignore, g, p, dz, s);
+  } else if (p.parts == 1 && one_wave(rows, V, N)) {
     launch_score_bwd<T, N, 4, 1>(m, rows, V, t, ignore, g, p, dz, s);
   } else {
     launch_score_bwd<T, N, 4, 4>(m, rows, V, t, ignore, g, p, dz, s);
@@ -1743,6 +1937,17 @@ void launch_distill(const Distill& a, const Upstream& up, T* dz) {
     hipLaunchKernelGGL((k_distill<T, N, U, W, false>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
 }
+template <typename T, int R, int W>
+void launch_step(const Distill& a, const Upstream& up, T* dz) {
+  constexpr int G = W == 1 ? 4 : 1;
+  const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
+  if (a.mix.two)
+    hipLaunchKernelGGL((k_distill_step<T, R, W, true>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       a.row_loss, a.stats, dz);
+  else
+    hipLaunchKernelGGL((k_distill_step<T, R, W, false>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+                       a.row_loss, a.stats, dz);
+}
 template <typename T, int N, int U, int W>
 void launch_distill_grad(const Distill& a, const Upstream& up, const Split& p, T* dz) {
   constexpr int G = 4 / W;
@@ -1764,8 +1969,8 @@ void distill_grad_any(const Distill& a, const Upstream& up, T* dz) {
   constexpr int N = Vec<T>::N;
   const Split p = map_split(a.rows, a.V);
   if (a.V <= SHORT_V) distill_short<T>(a, up, nullptr, dz);
-  else if (a.V <= 512) launch_distill_grad<T, 1, 8, 1>(a, up, p, dz);
-  else if (a.V <= 2048) launch_distill_grad<T, N, 4, 1>(a, up, p, dz);
+  else if (a.V <= 256) launch_distill_grad<T, 1, 4, 1>(a, up, p, dz);
+  else if (p.parts == 1 && one_wave(a.rows, a.V, N)) launch_distill_grad<T, N, 4, 1>(a, up, p, dz);
   else launch_distill_grad<T, N, 4, 4>(a, up, p, dz);
 }
 template <typename T>
@@ -1773,11 +1978,25 @@ void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) 
   constexpr int N = Vec<T>::N;
   T* dz = static_cast<T*>(dlogits);
   const Split p = row_split(a.rows, a.V);
+  const int nv = (a.V + N - 1) / N;
   if (a.V <= SHORT_V) {
     distill_short<T>(a, up, a.row_loss, dz);
-  } else if (a.V <= 512) {
-    launch_distill<T, 1, 8, 1>(a, up, dz);
-  } else if (a.V <= 2048) {
+  } else if (a.V <= 64) {
+    launch_distill<T, 1, 1, 1>(a, up, dz);
+  } else if (a.V <= 256) {
+    launch_distill<T, 1, 4, 1>(a, up, dz);
+  } else if (p.parts == 1 && dz && nv <= 16384) {
+    if (nv <= 64) launch_step<T, 1, 1>(a, up, dz);
+    else if (nv <= 128) launch_step<T, 2, 1>(a, up, dz);
+    else if (nv <= 256) launch_step<T, 4, 1>(a, up, dz);
+    else if (nv <= 1024) launch_step<T, 4, 4>(a, up, dz);
+    else if (nv <= 2048) launch_step<T, 8, 4>(a, up, dz);
+    else if (nv <= 4096) launch_step<T, 16, 4>(a, up, dz);
+    else if (nv <= 8192) launch_step<T, 16, 8>(a, up, dz);
+    else launch_step<T, 16, 16>(a, up, dz);
+  } else if (nv <= 64) {
+    launch_distill<T, N, 1, 1>(a, up, dz);
+  } else if (p.parts == 1 && one_wave(a.rows, a.V, N)) {
     launch_distill<T, N, 4, 1>(a, up, dz);
   } else if (p.parts == 1) {
     launch_distill<T, N, 4, 8>(a, up, dz);
