@@ -98,7 +98,8 @@ __device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
   if constexpr (N == 1) x[0] = to_f(*p);
   else unpack<T>(*reinterpret_cast<const typename Vec<T>::raw*>(p), x);
 }
-template <int N, typename T>
+// STREAM: past the caches (worth it for whole lines that nothing reads again soon)
+template <int N, bool STREAM = false, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   if constexpr (N == 1) {
     from_f(*p, x[0]);
@@ -108,7 +109,8 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
     for (int i = 0; i < N; ++i) from_f(e[i], x[i]);
     u32x4 v;
     __builtin_memcpy(&v, e, 16);
-    *reinterpret_cast<typename Vec<T>::raw*>(p) = v;
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T>::raw*>(p));
+    else *reinterpret_cast<typename Vec<T>::raw*>(p) = v;
   }
 }
 
@@ -649,7 +651,7 @@ inline Split row_split(int64_t rows, int64_t V) {
 }
 
 // f(value, index) over a row's values lo .. hi - 1, written to d: batches of U vectors
-template <typename T, int N, int U, int W, typename F>
+template <typename T, int N, int U, int W, bool STREAM, typename F>
 __device__ __forceinline__ void map_row(const T* z, T* d, int lo, int hi, int w, int lane, F f) {
   const int nv = (hi - lo) / N;
   constexpr int STEP = W * 64 * U;
@@ -663,7 +665,7 @@ __device__ __forceinline__ void map_row(const T* z, T* d, int lo, int hi, int w,
       if (v0 + u * W * 64 >= nv) break;
 #pragma unroll
       for (int i = 0; i < N; ++i) x[u][i] = f(x[u][i]);
-      store_vec<N>(d + lo + (v0 + u * W * 64) * N, x[u]);
+      store_vec<N, STREAM>(d + lo + (v0 + u * W * 64) * N, x[u]);
     }
   }
   if constexpr (N > 1) {
@@ -728,7 +730,7 @@ __global__ __launch_bounds__(256) void k_score_bwd(Rows rows, int64_t n_rows, in
   float top = 0.f;
   if (g.g_top) top = wave_sum(lane < g.top_k ? g.g_top[r * g.top_k + lane] : 0.f);
   const ScoreRow f = score_row(g, r, g1, top);
-  map_row<T, N, U, W>(z, d, lo, hi, w, lane, f);
+  map_row<T, N, U, W, false>(z, d, lo, hi, w, lane, f);
   group_sync<W>();
   if (w != 0) return;
   const int64_t id = g.g_top && lane < g.top_k ? g.top_id[r * g.top_k + lane] : -1;
@@ -1014,8 +1016,8 @@ __device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int h
     zero_row<T, N, W>(d, lo, hi, w, lane);
     return;
   }
-  if (g.two) map_row<T, N, U, W>(z, d, lo, hi, w, lane, [=](float x) { return g.both(x); });
-  else map_row<T, N, U, W>(z, d, lo, hi, w, lane, [=](float x) { return g.one(x); });
+  if (g.two) map_row<T, N, U, W, true>(z, d, lo, hi, w, lane, [=](float x) { return g.both(x); });
+  else map_row<T, N, U, W, true>(z, d, lo, hi, w, lane, [=](float x) { return g.one(x); });
   group_sync<W>();
   distill_entries<T, W>(z, d, lo, hi, tc, mix, g, lds, y, w, lane);
 }
@@ -1153,7 +1155,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
     unpack<T>(raw[u], x);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = TWO ? g.both(x[i]) : g.one(x[i]);
-    store_vec<N>(d + (v * N + N <= V ? v * N : V - N), x);
+    store_vec<N, true>(d + (v * N + N <= V ? v * N : V - N), x);
   }
   group_sync<W>();
   distill_entries<T, W>(z, d, 0, V, tc, mix, g, lds, y, w, lane);
@@ -1341,10 +1343,10 @@ __device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&x)
     for (int i = 0; i < VE; ++i) x[i] = c + i < D ? to_f(row[c + i]) : 0.f;
   }
 }
-template <typename T, int VE>
+template <typename T, int VE, bool STREAM = false>
 __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&x)[VE]) {
   if (D >= VE) {
-    store_vec<VE>(row + c, x);
+    store_vec<VE, STREAM>(row + c, x);
   } else {
 #pragma unroll
     for (int i = 0; i < VE; ++i)
@@ -1353,7 +1355,7 @@ __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&x
 }
 
 // A block takes `per` rows of `vecs` vectors; lanes take vectors in turn.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict__ weight, int64_t w_stride,
                                                     float scale, T* __restrict__ out, int64_t N, int64_t V, int D,
                                                     int vecs, int per) {
@@ -1377,7 +1379,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
       const float f = v[u] >= 0 && v[u] < V ? scale : __builtin_nanf("");
 #pragma unroll
       for (int i = 0; i < VE; ++i) x[u][i] *= f;
-      store_cols<T, VE>(out + (i0 + t / vecs) * D, edge_col<VE>(t % vecs * VE, D), D, x[u]);
+      store_cols<T, VE, STREAM>(out + (i0 + t / vecs) * D, edge_col<VE>(t % vecs * VE, D), D, x[u]);
     }
   }
 }
@@ -1616,7 +1618,7 @@ __global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes,
 // 64 / lpr chunks per wave.  A token inside the chunk is finished here; one that goes on
 // from the chunk before leaves its sum in parts[c][0], one that begins here and goes on
 // after it in parts[c][1].  Blocks past the chunks clear table rows without a token.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
                                                     uint32_t none, const T* __restrict__ dout, int64_t d_stride,
                                                     float scale, T* __restrict__ dw, int64_t N, int D, int chunk,
@@ -1631,7 +1633,7 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
     for (int64_t v = v0 + (threadIdx.x >> 6); v < v1; v += 4)
       if (!used[v])
         for (int c = (threadIdx.x & 63) * VE; c < D; c += 64 * VE)
-          store_cols<T, VE>(dw + v * D, edge_col<VE>(c, D), D, zero);
+          store_cols<T, VE, STREAM>(dw + v * D, edge_col<VE>(c, D), D, zero);
     return;
   }
   const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / lpr;
@@ -1661,7 +1663,7 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
     } else {
 #pragma unroll
       for (int i = 0; i < VE; ++i) acc[i] *= scale;
-      store_cols<T, VE>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
+      store_cols<T, VE, STREAM>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
     }
   };
   // keys and positions of the next step are read ahead (16 bytes each: chunks are multiples
@@ -1985,21 +1987,21 @@ void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) 
     launch_distill<T, 1, 1, 1>(a, up, dz);
   } else if (a.V <= 256) {
     launch_distill<T, 1, 4, 1>(a, up, dz);
-  } else if (p.parts == 1 && dz && nv <= 16384) {
+  } else if (p.parts == 1 && dz && nv <= 4096) {
     if (nv <= 64) launch_step<T, 1, 1>(a, up, dz);
     else if (nv <= 128) launch_step<T, 2, 1>(a, up, dz);
     else if (nv <= 256) launch_step<T, 4, 1>(a, up, dz);
     else if (nv <= 1024) launch_step<T, 4, 4>(a, up, dz);
     else if (nv <= 2048) launch_step<T, 8, 4>(a, up, dz);
-    else if (nv <= 4096) launch_step<T, 16, 4>(a, up, dz);
-    else if (nv <= 8192) launch_step<T, 16, 8>(a, up, dz);
-    else launch_step<T, 16, 16>(a, up, dz);
+    else launch_step<T, 16, 4>(a, up, dz);
   } else if (nv <= 64) {
     launch_distill<T, N, 1, 1>(a, up, dz);
   } else if (p.parts == 1 && one_wave(a.rows, a.V, N)) {
     launch_distill<T, N, 4, 1>(a, up, dz);
-  } else if (p.parts == 1) {
+  } else if (p.parts == 1 && !(dz && nv > 8192)) {
     launch_distill<T, N, 4, 8>(a, up, dz);
+  } else if (p.parts == 1) {
+    launch_distill<T, N, 4, 16>(a, up, dz);
   } else {
     float4* sums = reinterpret_cast<float4*>(static_cast<char*>(ws) + DISTILL_WS_HEAD);
     const dim3 g(static_cast<unsigned>(a.rows * p.parts)), g1(static_cast<unsigned>(a.rows));
@@ -2085,6 +2087,15 @@ extern "C" int ghm_distill_bwd(const void* logits, int dtype, int64_t n_inner, i
   GHM_CHECK(N >= 0 && N < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31) && D >= 1 && D <= (int64_t(1) << 20), \
             "shape (N, V < 2^31, D <= 2^20)")
 
+namespace {
+// rows of whole 64-byte lines are stored past the caches: the gradient of 16,384 x 2048
+// bf16 tokens into 65,536 rows took 98 us that way and 114 us through them; rows that share
+// lines (1001 f32 values) 164 us and 163 us
+inline bool whole_lines(const void* p, int64_t row_bytes) {
+  return reinterpret_cast<uintptr_t>(p) % 64 == 0 && row_bytes % 64 == 0;
+}
+}  // namespace
+
 extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* weight, int dtype, int64_t w_stride,
                                   float scale, void* out, int64_t N, int64_t V, int64_t D, void* stream) {
   EMBED_CHECK();
@@ -2093,9 +2104,16 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
   if (N == 0) return GHM_OK;
   const int ve = dtype == 0 ? 4 : 8, vecs = static_cast<int>((D + ve - 1) / ve);
   const int per = vecs >= 1024 ? 1 : 1024 / vecs;
-  TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_rows<T>, dim3(static_cast<unsigned>((N + per - 1) / per)), dim3(256), 0,
-                                         ghm_stream(stream), Ids{tokens, id_bits}, static_cast<const T*>(weight),
-                                         w_stride, scale, static_cast<T*>(out), N, V, static_cast<int>(D), vecs, per));
+  const dim3 g(static_cast<unsigned>((N + per - 1) / per)), b(256);
+  const Ids t{tokens, id_bits};
+  const int d = static_cast<int>(D);
+  hipStream_t s = ghm_stream(stream);
+  if (whole_lines(out, D * (16 / ve)))
+    TOK_DISPATCH(dtype, hipLaunchKernelGGL((k_embed_rows<T, true>), g, b, 0, s, t, static_cast<const T*>(weight), w_stride,
+                                           scale, static_cast<T*>(out), N, V, d, vecs, per));
+  else
+    TOK_DISPATCH(dtype, hipLaunchKernelGGL((k_embed_rows<T, false>), g, b, 0, s, t, static_cast<const T*>(weight),
+                                           w_stride, scale, static_cast<T*>(out), N, V, d, vecs, per));
   return ghm_launch_status();
 }
 
@@ -2191,9 +2209,14 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
   if (rpb > 4096) rpb = 4096;
   while ((V + rpb - 1) / rpb > (1 << 20)) rpb *= 2;
   const int64_t zero_blocks = (V + rpb - 1) / rpb;
-  hipLaunchKernelGGL(k_embed_sums<T>, dim3(static_cast<unsigned>(sum_blocks + zero_blocks)), dim3(256), 0, s, key, pos,
-                     static_cast<uint32_t>(V), dout, d_stride, scale, dw, N, D, p.chunk, p.chunks, p.slices, p.lpr,
-                     sum_blocks, parts, used, V, static_cast<int>(rpb));
+  const dim3 g(static_cast<unsigned>(sum_blocks + zero_blocks)), b(256);
+  const uint32_t none = static_cast<uint32_t>(V);
+  if (whole_lines(dw, D * static_cast<int64_t>(sizeof(T))))
+    hipLaunchKernelGGL((k_embed_sums<T, true>), g, b, 0, s, key, pos, none, dout, d_stride, scale, dw, N, D, p.chunk,
+                       p.chunks, p.slices, p.lpr, sum_blocks, parts, used, V, static_cast<int>(rpb));
+  else
+    hipLaunchKernelGGL((k_embed_sums<T, false>), g, b, 0, s, key, pos, none, dout, d_stride, scale, dw, N, D, p.chunk,
+                       p.chunks, p.slices, p.lpr, sum_blocks, parts, used, V, static_cast<int>(rpb));
   if (p.chunks > 1)
     hipLaunchKernelGGL(k_embed_join<T>, dim3(static_cast<unsigned>(p.chunks - 1), static_cast<unsigned>((D + 255) / 256)),
                        dim3(256), 0, s, key, static_cast<uint32_t>(V), scale, dw, N, D, p.chunk, p.chunks, parts);
