@@ -1391,8 +1391,10 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
 // rows without a token are written 0 beside it.  No atomics on values: a fixed order.
 // ---------------------------------------------------------------------------
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_ROUNDS = 8;
-constexpr int SORT_TILES = 128;  // up to this many tiles a block sums their counts itself
+constexpr int SORT_SELF_N = 16384;  // up to this many positions a block counts them all itself
+constexpr int SORT_TILES = 128;     // up to this many tiles it sums their counts itself
 
+__device__ __forceinline__ uint32_t digit(uint32_t key, int shift, int bits) { return (key >> shift) & ((1u << bits) - 1); }
 // The sorted key of a position is its token, or `none` for a token that gets no gradient.
 struct SortIn {  // the first pass reads tokens, later ones the previous pass's keys and positions
   Ids tok;
@@ -1415,24 +1417,31 @@ __device__ __forceinline__ void sort_in(const SortIn& in, int64_t i, int64_t ste
   }
 }
 
-// counts[tile][digit]; the first pass also clears the table of rows that have a token
+// Table rows that have a token, one byte each: cleared by the first launch of a sort and set
+// by a later one.
+__device__ __forceinline__ void clear_used(uint32_t* used, int64_t words, int threads) {
+  if (used)
+    for (int64_t j = static_cast<int64_t>(blockIdx.x) * threads + threadIdx.x; j < words;
+         j += static_cast<int64_t>(gridDim.x) * threads)
+      used[j] = 0;
+}
+
+// counts[tile][digit]
 template <int W>
-__global__ __launch_bounds__(64 * W) void k_sort_count(SortIn in, int64_t N, int shift, uint32_t* __restrict__ counts,
+__global__ __launch_bounds__(64 * W) void k_sort_count(SortIn in, int64_t N, int shift, int bits,
+                                                       uint32_t* __restrict__ counts,
                                                        uint32_t* __restrict__ used, int64_t used_words) {
   __shared__ uint32_t bins[SORT_BINS];
   constexpr int TILE = 64 * W * SORT_ROUNDS;
   for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) bins[d] = 0;
-  if (used)
-    for (int64_t j = static_cast<int64_t>(blockIdx.x) * 64 * W + threadIdx.x; j < used_words;
-         j += static_cast<int64_t>(gridDim.x) * 64 * W)
-      used[j] = 0;
+  clear_used(used, used_words, 64 * W);
   __syncthreads();
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * TILE + threadIdx.x;
   uint32_t key[SORT_ROUNDS];
   sort_in<SORT_ROUNDS>(in, i0, 64 * W, N, key);
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q)
-    if (i0 + q * 64 * W < N) atomicAdd(&bins[(key[q] >> shift) & (SORT_BINS - 1)], 1u);
+    if (i0 + q * 64 * W < N) atomicAdd(&bins[digit(key[q], shift, bits)], 1u);
   __syncthreads();
   for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d] = bins[d];
 }
@@ -1448,25 +1457,59 @@ __global__ __launch_bounds__(64) void k_sort_scan(uint32_t* __restrict__ counts,
   }
   c[tiles * SORT_BINS] = s;
 }
-// Positions go to: start of the digit + the digit's count in earlier tiles + in earlier
-// waves + in this wave's earlier rounds + among lower lanes.  A wave takes 64 * SORT_ROUNDS
-// consecutive positions, so the sort is stable.
-template <int W>
-__global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, int shift,
-                                                         const uint32_t* __restrict__ counts, int tiles, int scanned,
+// One pass: positions go to the start of their digit + the digit's count in earlier tiles +
+// in earlier waves + in this wave's earlier rounds + among lower lanes.  A wave takes
+// 64 * SORT_ROUNDS consecutive positions, so the sort is stable.  The counts per tile come
+// from k_sort_count: summed here (SORT_SUM) or by k_sort_scan (SORT_SCANNED); for few
+// positions each block counts all of them itself (SORT_SELF: one launch instead of two).
+enum { SORT_SUM, SORT_SCANNED, SORT_SELF };
+template <int W, int MODE>
+__global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, int shift, int bits,
+                                                         const uint32_t* __restrict__ counts, int tiles,
                                                          uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
-                                                         uint8_t* __restrict__ used) {
+                                                         uint8_t* __restrict__ set_used, int one_pass,
+                                                         uint32_t* __restrict__ clear, int64_t used_words) {
   __shared__ uint32_t wbins[W][SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 64];
+  __shared__ uint32_t self[MODE == SORT_SELF ? 2 : 1][MODE == SORT_SELF ? SORT_BINS : 1];
+  constexpr int TILE = 64 * W * SORT_ROUNDS;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * W + w) * 64 * SORT_ROUNDS + lane;
+  uint32_t key[SORT_ROUNDS], at[SORT_ROUNDS], pos[SORT_ROUNDS];
+  sort_in<SORT_ROUNDS>(in, i0, 64, N, key);
+#pragma unroll
+  for (int q = 0; q < SORT_ROUNDS; ++q) {
+    const int64_t i = i0 + q * 64;
+    pos[q] = in.pos ? in.pos[i < N ? i : N - 1] : static_cast<uint32_t>(i);
+  }
   for (int d = lane; d < SORT_BINS; d += 64) wbins[w][d] = 0;
+  clear_used(clear, used_words, 64 * W);
+  if constexpr (MODE == SORT_SELF) {
+    for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) self[0][d] = self[1][d] = 0;
+    __syncthreads();
+    for (int64_t t0 = 0; t0 < N; t0 += 2 * TILE) {
+      uint32_t k[2 * SORT_ROUNDS];
+      sort_in<2 * SORT_ROUNDS>(in, t0 + threadIdx.x, 64 * W, N, k);
+#pragma unroll
+      for (int q = 0; q < 2 * SORT_ROUNDS; ++q) {
+        const int64_t i = t0 + threadIdx.x + q * 64 * W;
+        const uint32_t d = digit(k[q], shift, bits);
+        if (i < N) atomicAdd(&self[i < static_cast<int64_t>(blockIdx.x) * TILE ? 0 : 1][d], 1u);
+      }
+    }
+    __syncthreads();
+  }
   // digit totals and the counts of earlier tiles; then an exclusive scan over the digits
   for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
     uint32_t before = 0, all = 0;
-    if (scanned) {
+    if constexpr (MODE == SORT_SELF) {
+      before = self[0][d];
+      all = before + self[1][d];
+      if (one_pass && blockIdx.x == 0 && d < static_cast<int64_t>(in.none)) set_used[d] = all != 0;
+    } else if constexpr (MODE == SORT_SCANNED) {
       before = counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d];
       all = counts[static_cast<int64_t>(tiles) * SORT_BINS + d];
     } else {
-#pragma unroll 8
+#pragma unroll 16
       for (int t = 0; t < tiles; ++t) {
         const uint32_t c = counts[t * SORT_BINS + d];
         before += t < static_cast<int>(blockIdx.x) ? c : 0;
@@ -1488,21 +1531,12 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
     for (int j = 0; j < d >> 6; ++j) s += wsum[j];
     base[d] = s;
   }
-  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * W + w) * 64 * SORT_ROUNDS + lane;
-  uint32_t key[SORT_ROUNDS], at[SORT_ROUNDS], pos[SORT_ROUNDS];
-  sort_in<SORT_ROUNDS>(in, i0, 64, N, key);
-#pragma unroll
-  for (int q = 0; q < SORT_ROUNDS; ++q) {
-    const int64_t i = i0 + q * 64;
-    pos[q] = in.pos ? in.pos[i < N ? i : N - 1] : static_cast<uint32_t>(i);
-  }
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
     const bool live = i0 + q * 64 < N;
-    const uint32_t d = (key[q] >> shift) & (SORT_BINS - 1);
+    const uint32_t d = digit(key[q], shift, bits);
     uint64_t same = __ballot(live);
-#pragma unroll
-    for (int bit = 0; bit < SORT_BITS; ++bit) {
+    for (int bit = 0; bit < bits; ++bit) {
       const uint64_t m = __ballot((d >> bit) & 1);
       same &= (d >> bit) & 1 ? m : ~m;
     }
@@ -1516,19 +1550,18 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
     if (i0 + q * 64 >= N) break;
-    const uint32_t d = (key[q] >> shift) & (SORT_BINS - 1);
+    const uint32_t d = digit(key[q], shift, bits);
     uint32_t to = base[d] + at[q];
     for (int j = 0; j < w; ++j) to += wbins[j][d];
     key_out[to] = key[q];
     pos_out[to] = pos[q];
-    if (used && key[q] != in.none) used[key[q]] = 1;
+    if (set_used && !one_pass && key[q] != in.none) set_used[key[q]] = 1;
   }
 }
 
 // Up to SORT_ONE positions of a table of at most USED_ONE rows: all passes by one block,
 // key and position in one word of LDS between them.
-constexpr int POS_BITS = 14, SORT_ONE = 1 << POS_BITS, USED_ONE = (1 << (32 - POS_BITS)) - 1;
-template <int ROUNDS>
+constexpr int ROUNDS = 4, POS_BITS = 12, SORT_ONE = 1 << POS_BITS, USED_ONE = (1 << (32 - POS_BITS)) - 1;
 __global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes, int bits, uint32_t* __restrict__ key_out,
                                                    uint32_t* __restrict__ pos_out, uint32_t* __restrict__ used,
                                                    int used_words) {
@@ -1552,10 +1585,9 @@ __global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes,
     wave_fence();  // a wave ranks the words that it wrote, or that a barrier has passed
     for (int i = i0; i - lane < N && i < i0 + 64 * ROUNDS; i += 64) {
       const bool live = i < N;
-      const uint32_t d = live ? (word[i] >> shift) & (SORT_BINS - 1) : 0;
+      const uint32_t d = live ? digit(word[i], shift, bits) : 0;
       uint64_t same = __ballot(live);
-#pragma unroll
-      for (int bit = 0; bit < SORT_BITS; ++bit) {
+      for (int bit = 0; bit < bits; ++bit) {
         const uint64_t m = __ballot((d >> bit) & 1);
         same &= (d >> bit) & 1 ? m : ~m;
       }
@@ -1594,7 +1626,7 @@ __global__ __launch_bounds__(1024) void k_sort_one(SortIn in, int N, int passes,
     for (int q = 0; q < ROUNDS; ++q) {
       const int i = i0 + q * 64;
       x[q] = i < N ? word[i] : 0;
-      const uint32_t d = (x[q] >> shift) & (SORT_BINS - 1);
+      const uint32_t d = digit(x[q], shift, bits);
       to[q] = i < N ? base[d] + wbins[w][d] + rank[i] : 0;
       if (p == 0 && i < N && x[q] >> POS_BITS != in.none)
         reinterpret_cast<uint8_t*>(used)[x[q] >> POS_BITS] = 1;  // cleared before the barriers
@@ -2119,9 +2151,8 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
 
 namespace {
 struct EmbedPlan {
-  int W, passes, bits, chunk, slices, lpr;
-  bool one;
-  int64_t tiles, chunks, used_words;
+  int passes, bits, chunk, slices, lpr;
+  int64_t chunks, used_words;
   int64_t key[2], pos[2], counts, used, parts, bytes;  // byte offsets in the workspace
 };
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -2131,10 +2162,6 @@ inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
   while (bits < 32 && (int64_t(1) << bits) <= V) ++bits;  // keys 0 .. V
   p.passes = (bits + SORT_BITS - 1) / SORT_BITS;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.W = N <= 64 * 4 * SORT_ROUNDS * SORT_TILES ? 4 : 16;
-  p.one = N <= SORT_ONE && V <= USED_ONE;
-  const int64_t tile = 64 * p.W * SORT_ROUNDS;
-  p.tiles = (N + tile - 1) / tile;
   p.lpr = 1;
   while (p.lpr < 64 && p.lpr * ve < D) p.lpr *= 2;
   p.slices = static_cast<int>((D + p.lpr * ve - 1) / (p.lpr * ve));
@@ -2148,32 +2175,34 @@ inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
     p.key[i] = at, at += up256(N * 4);
     p.pos[i] = at, at += up256(N * 4);
   }
-  p.counts = at, at += up256((p.tiles + 1) * SORT_BINS * 4);
+  p.counts = at, at += up256((N / (64 * 4 * SORT_ROUNDS) + 2) * SORT_BINS * 4);
   p.used = at, at += up256(p.used_words * 4);
   p.parts = at, at += up256(p.chunks * 2 * D * 4);
   p.bytes = at;
   return p;
 }
 
-template <int W>
+template <int W, int MODE>
 void launch_sort(const EmbedPlan& p, const Ids& tok, int64_t pad, int64_t N, int64_t V, char* ws, hipStream_t s) {
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
   uint32_t* used = reinterpret_cast<uint32_t*>(ws + p.used);
-  const dim3 g(static_cast<unsigned>(p.tiles)), b(64 * W);
-  const int scanned = p.tiles > SORT_TILES;
+  const int64_t tile = 64 * W * SORT_ROUNDS, tiles = (N + tile - 1) / tile;
+  const dim3 g(static_cast<unsigned>(tiles)), b(64 * W);
   for (int i = 0; i < p.passes; ++i) {
     SortIn in{tok, nullptr, nullptr, pad, static_cast<uint32_t>(V)};
     if (i > 0) {
       in.key = reinterpret_cast<uint32_t*>(ws + p.key[(i - 1) & 1]);
       in.pos = reinterpret_cast<uint32_t*>(ws + p.pos[(i - 1) & 1]);
     }
-    // a digit has SORT_BITS bits; the passes are p.bits apart, so digits may overlap by
-    // bits that an earlier pass has sorted already
-    hipLaunchKernelGGL(k_sort_count<W>, g, b, 0, s, in, N, i * p.bits, counts, i == 0 ? used : nullptr, p.used_words);
-    if (scanned) hipLaunchKernelGGL(k_sort_scan, dim3(SORT_BINS / 64), dim3(64), 0, s, counts, p.tiles);
-    hipLaunchKernelGGL(k_sort_scatter<W>, g, b, 0, s, in, N, i * p.bits, counts, static_cast<int>(p.tiles), scanned,
+    if (MODE != SORT_SELF)
+      hipLaunchKernelGGL(k_sort_count<W>, g, b, 0, s, in, N, i * p.bits, p.bits, counts, i == 0 ? used : nullptr, p.used_words);
+    if (MODE == SORT_SCANNED) hipLaunchKernelGGL(k_sort_scan, dim3(SORT_BINS / 64), dim3(64), 0, s, counts, tiles);
+    // cleared by the first launch, set by the second; a single one writes every row's from its counts
+    const bool one_pass = MODE == SORT_SELF && p.passes == 1, clear = MODE == SORT_SELF && i == 0 && !one_pass;
+    const bool set = MODE == SORT_SELF ? one_pass || i == 1 : i == 0;
+    hipLaunchKernelGGL((k_sort_scatter<W, MODE>), g, b, 0, s, in, N, i * p.bits, p.bits, counts, static_cast<int>(tiles),
                        reinterpret_cast<uint32_t*>(ws + p.key[i & 1]), reinterpret_cast<uint32_t*>(ws + p.pos[i & 1]),
-                       i == 0 ? reinterpret_cast<uint8_t*>(used) : nullptr);
+                       set ? reinterpret_cast<uint8_t*>(used) : nullptr, one_pass, clear ? used : nullptr, p.used_words);
   }
 }
 template <typename T>
@@ -2187,18 +2216,16 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
   const EmbedPlan p = embed_plan(N, V, D, Vec<T>::N);
   uint32_t* key = reinterpret_cast<uint32_t*>(ws + p.key[(p.passes - 1) & 1]);
   uint32_t* pos = reinterpret_cast<uint32_t*>(ws + p.pos[(p.passes - 1) & 1]);
-  if (p.one) {
+  if (N <= SORT_ONE && V <= USED_ONE) {
     const SortIn in{tok, nullptr, nullptr, pad, static_cast<uint32_t>(V)};
-    uint32_t* flags = reinterpret_cast<uint32_t*>(ws + p.used);
-    const int n = static_cast<int>(N), words = static_cast<int>(p.used_words);
-    if (N <= 4096)
-      hipLaunchKernelGGL(k_sort_one<4>, dim3(1), dim3(1024), 0, s, in, n, p.passes, p.bits, key, pos, flags, words);
-    else
-      hipLaunchKernelGGL(k_sort_one<16>, dim3(1), dim3(1024), 0, s, in, n, p.passes, p.bits, key, pos, flags, words);
-  } else if (p.W == 4) {
-    launch_sort<4>(p, tok, pad, N, V, ws, s);
+    hipLaunchKernelGGL(k_sort_one, dim3(1), dim3(1024), 0, s, in, static_cast<int>(N), p.passes, p.bits, key, pos,
+                       reinterpret_cast<uint32_t*>(ws + p.used), static_cast<int>(p.used_words));
+  } else if (N <= SORT_SELF_N) {
+    launch_sort<8, SORT_SELF>(p, tok, pad, N, V, ws, s);
+  } else if (N <= 64 * 4 * SORT_ROUNDS * SORT_TILES) {
+    launch_sort<4, SORT_SUM>(p, tok, pad, N, V, ws, s);
   } else {
-    launch_sort<16>(p, tok, pad, N, V, ws, s);
+    launch_sort<16, SORT_SCANNED>(p, tok, pad, N, V, ws, s);
   }
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   const uint8_t* used = reinterpret_cast<uint8_t*>(ws + p.used);
