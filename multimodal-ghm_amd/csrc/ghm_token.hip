@@ -1469,8 +1469,14 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
                                                          uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
                                                          uint8_t* __restrict__ set_used, int one_pass,
                                                          uint32_t* __restrict__ clear, int64_t used_words) {
+  // SORT_SUM: groups of 128 threads take 4 digits each of every GROUPS-th tile
+  constexpr int GROUPS = MODE == SORT_SUM ? W / 2 : 1;
+  __shared__ uint32_t tsum[2][GROUPS][MODE == SORT_SUM ? SORT_BINS : 1];
+  // equal digits of a wave meet at one of SPREAD counters (64 lanes of 10 tokens at one each
+  // took 14 us for 10,368 positions)
+  constexpr int SPREAD = MODE == SORT_SELF ? 8 : 1;
   __shared__ uint32_t wbins[W][SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 64];
-  __shared__ uint32_t self[MODE == SORT_SELF ? 2 : 1][MODE == SORT_SELF ? SORT_BINS : 1];
+  __shared__ uint32_t self[2][MODE == SORT_SELF ? SORT_BINS * SPREAD : 1];
   constexpr int TILE = 64 * W * SORT_ROUNDS;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * W + w) * 64 * SORT_ROUNDS + lane;
@@ -1484,7 +1490,7 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
   for (int d = lane; d < SORT_BINS; d += 64) wbins[w][d] = 0;
   clear_used(clear, used_words, 64 * W);
   if constexpr (MODE == SORT_SELF) {
-    for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) self[0][d] = self[1][d] = 0;
+    for (int d = threadIdx.x; d < SORT_BINS * SPREAD; d += 64 * W) self[0][d] = self[1][d] = 0;
     __syncthreads();
     for (int64_t t0 = 0; t0 < N; t0 += 2 * TILE) {
       uint32_t k[2 * SORT_ROUNDS];
@@ -1492,44 +1498,24 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
 #pragma unroll
       for (int q = 0; q < 2 * SORT_ROUNDS; ++q) {
         const int64_t i = t0 + threadIdx.x + q * 64 * W;
-        const uint32_t d = digit(k[q], shift, bits);
+        const uint32_t d = digit(k[q], shift, bits) * SPREAD + lane % SPREAD;
         if (i < N) atomicAdd(&self[i < static_cast<int64_t>(blockIdx.x) * TILE ? 0 : 1][d], 1u);
       }
     }
-    __syncthreads();
+  } else {
+    wave_fence();
   }
-  // digit totals and the counts of earlier tiles; then an exclusive scan over the digits
-  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
-    uint32_t before = 0, all = 0;
-    if constexpr (MODE == SORT_SELF) {
-      before = self[0][d];
-      all = before + self[1][d];
-      if (one_pass && blockIdx.x == 0 && d < static_cast<int64_t>(in.none)) set_used[d] = all != 0;
-    } else if constexpr (MODE == SORT_SCANNED) {
-      before = counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d];
-      all = counts[static_cast<int64_t>(tiles) * SORT_BINS + d];
-    } else {
+  if constexpr (MODE == SORT_SUM) {
+    u32x4 before = {}, all = {};
+    const int d = (threadIdx.x & 127) * 4;
 #pragma unroll 16
-      for (int t = 0; t < tiles; ++t) {
-        const uint32_t c = counts[t * SORT_BINS + d];
-        before += t < static_cast<int>(blockIdx.x) ? c : 0;
-        all += c;
-      }
+    for (int t = threadIdx.x >> 7; t < tiles; t += GROUPS) {
+      const u32x4 c = *reinterpret_cast<const u32x4*>(counts + t * SORT_BINS + d);
+      before += t < static_cast<int>(blockIdx.x) ? c : u32x4{};
+      all += c;
     }
-    uint32_t inc = all;  // 64 consecutive digits per wave
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t up = __shfl_up(inc, o, 64);
-      inc += lane >= o ? up : 0;
-    }
-    if (lane == 63) wsum[d >> 6] = inc;
-    base[d] = inc - all + before;
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
-    uint32_t s = base[d];
-    for (int j = 0; j < d >> 6; ++j) s += wsum[j];
-    base[d] = s;
+    *reinterpret_cast<u32x4*>(&tsum[0][threadIdx.x >> 7][d]) = before;
+    *reinterpret_cast<u32x4*>(&tsum[1][threadIdx.x >> 7][d]) = all;
   }
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
@@ -1547,12 +1533,51 @@ __global__ __launch_bounds__(64 * W) void k_sort_scatter(SortIn in, int64_t N, i
     wave_fence();
   }
   __syncthreads();
+  // counts become starts: over the waves, over earlier tiles, and by a scan over the digits
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t c = wbins[j][d];
+      wbins[j][d] = mine;
+      mine += c;
+    }
+    uint32_t before = 0, all = 0;
+    if constexpr (MODE == SORT_SELF) {
+#pragma unroll
+      for (int j = 0; j < SPREAD; ++j) {
+        before += self[0][d * SPREAD + j];
+        all += self[1][d * SPREAD + j];
+      }
+      all += before;
+      if (one_pass && blockIdx.x == 0 && d < static_cast<int64_t>(in.none)) set_used[d] = all != 0;
+    } else if constexpr (MODE == SORT_SCANNED) {
+      before = counts[static_cast<int64_t>(blockIdx.x) * SORT_BINS + d];
+      all = counts[static_cast<int64_t>(tiles) * SORT_BINS + d];
+    } else {
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        before += tsum[0][j][d];
+        all += tsum[1][j][d];
+      }
+    }
+    uint32_t inc = all;  // 64 consecutive digits per wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up(inc, o, 64);
+      inc += lane >= o ? up : 0;
+    }
+    if (lane == 63) wsum[d >> 6] = inc;
+    base[d] = inc - all + before;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < SORT_BINS; d += 64 * W)
+    for (int j = 0; j < d >> 6; ++j) base[d] += wsum[j];
+  __syncthreads();
 #pragma unroll
   for (int q = 0; q < SORT_ROUNDS; ++q) {
     if (i0 + q * 64 >= N) break;
-    const uint32_t d = digit(key[q], shift, bits);
-    uint32_t to = base[d] + at[q];
-    for (int j = 0; j < w; ++j) to += wbins[j][d];
+    const uint32_t d = digit(key[q], shift, bits), to = base[d] + wbins[w][d] + at[q];
     key_out[to] = key[q];
     pos_out[to] = pos[q];
     if (set_used && !one_pass && key[q] != in.none) set_used[key[q]] = 1;
@@ -1698,32 +1723,53 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
       store_cols<T, VE, STREAM>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
     }
   };
-  // keys and positions of the next step are read ahead (16 bytes each: chunks are multiples
-  // of U, and the arrays are padded); entries past the end take row 0 and are not used
+  // Rows are read one step ahead of their sums and kept packed, keys and positions two steps
+  // (16 bytes each: chunks are multiples of U, and the arrays are padded).  Entries past
+  // the end take row 0 and are not used; short rows (D < VE) go without the pipeline.
   static_assert(U == 8, "two 16-byte reads per step");
-  u32x4 kn[2], pn[2];
-  const auto ahead = [&](int64_t i) {
+  u32x4 kn[2], pn[2], row[U];
+  uint32_t k[U];
+  const auto ids = [&](int64_t i) {
+    if (i >= hi) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       kn[h] = reinterpret_cast<const u32x4*>(key + i)[h];
       pn[h] = reinterpret_cast<const u32x4*>(pos + i)[h];
     }
   };
-  ahead(lo);
+  const auto rows = [&](int64_t i) {
+    if (i >= hi) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = i + u < hi ? pn[u / 4][u % 4] : 0;
+      if (D >= VE) {
+        row[u] = *reinterpret_cast<const typename Vec<T>::raw*>(dout + r * d_stride + col);
+      } else {
+        T e[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) e[j] = dout[r * d_stride + (j < D ? j : D - 1)];
+        __builtin_memcpy(&row[u], e, 16);
+      }
+    }
+  };
+  ids(lo);
+  rows(lo);
   for (int64_t i = lo; i < hi; i += U) {
-    uint32_t k[U];
     float x[U][VE];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       k[u] = kn[u / 4][u % 4];
-      const int64_t row = i + u < hi ? pn[u / 4][u % 4] : 0;
-      load_cols<T, VE>(dout + row * d_stride, col, D, x[u]);
     }
     if (k[0] == none) break;  // only tokens without a gradient follow
-    if (i + U < hi) ahead(i + U);
+    ids(i + U);
+    u32x4 now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = row[u];
+    rows(i + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= hi) break;
+      unpack<T>(now[u], x[u]);
       if (k[u] != cur) {
         flush(false);
         cur = k[u];
