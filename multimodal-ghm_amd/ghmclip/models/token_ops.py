@@ -45,7 +45,7 @@ def _ids(t, shape, device, what, bits=(8, 32, 64)):
     if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, the logits on {device}")
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
     return t.contiguous(), _ID_BITS[t.dtype]
 
 
@@ -100,14 +100,23 @@ def _check_logits(logits):
     return code
 
 
+def _first_order(backward):
+    """A backward that is not itself differentiable: torch's wrapper refuses a second
+    gradient; it is only entered where a graph of the backward is built (4 us a call)."""
+    refusing = torch.autograd.function.once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(either)
+
+
 # ---- scores ---------------------------------------------------------------
 
 
-def _score(logits, targets, top_k, ignore_index, want_stats):
+def _score(logits, y, bits, top_k, ignore_index, want_stats):
     code, dev, lead, V = _DTYPE[logits.dtype], logits.device, logits.shape[:-1], logits.shape[-1]
     z, n_inner, so, si = _rows(logits)
     rows = logits.numel() // V
-    y, bits = (None, 64) if targets is None else _ids(targets, lead, dev, "targets")
     logprob = None if y is None else torch.empty(lead, dtype=torch.float32, device=dev)
     entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
@@ -122,30 +131,29 @@ def _score(logits, targets, top_k, ignore_index, want_stats):
 
 class _ScoreFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, top_k, ignore_index):
-        logprob, entropy, top_lp, top_id, stats = _score(logits, targets, top_k, ignore_index, True)
+    def forward(ctx, logits, y, bits, top_k, ignore_index):
+        logprob, entropy, top_lp, top_id, stats = _score(logits, y, bits, top_k, ignore_index, True)
         ctx.set_materialize_grads(False)
-        ctx.top_k, ctx.ignore_index = top_k, ignore_index
-        ctx.save_for_backward(logits, targets, entropy, top_id, stats)
+        ctx.args = bits, top_k, ignore_index
+        ctx.save_for_backward(logits, y, entropy, top_id, stats)
         if top_id is not None:
             ctx.mark_non_differentiable(top_id)
         return logprob, entropy, top_lp, top_id
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g_lp, g_ent, g_top, _g_id):
         if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None
-        logits, targets, entropy, top_id, stats = ctx.saved_tensors
+            return None, None, None, None, None
+        logits, y, entropy, top_id, stats = ctx.saved_tensors
+        bits, top_k, ignore_index = ctx.args
         dev, V = logits.device, logits.shape[-1]
         z, n_inner, so, si = _rows(logits)
-        y, bits = (None, 64) if targets is None else _ids(targets, logits.shape[:-1], dev, "targets")
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         _call(dev, "ghm_token_logprobs_bwd", z.data_ptr(), _DTYPE[logits.dtype], n_inner, so, si, logits.numel() // V,
-              V, _ptr(y), bits, ctx.ignore_index, ctx.top_k, _ptr(top_id), stats.data_ptr(), entropy.data_ptr(),
-              _ptr(g_lp), _ptr(g_ent), _ptr(g_top), dz.data_ptr())
-        return dz, None, None, None
+              V, _ptr(y), bits, ignore_index, top_k, _ptr(top_id), stats.data_ptr(), entropy.data_ptr(), _ptr(g_lp),
+              _ptr(g_ent), _ptr(g_top), dz.data_ptr())
+        return dz, None, None, None, None
 
 
 def token_logprobs(logits, targets=None, top_k=0, ignore_index=-100):
@@ -164,37 +172,43 @@ def token_logprobs(logits, targets=None, top_k=0, ignore_index=-100):
     _check_logits(logits)
     if not isinstance(top_k, int) or not 0 <= top_k <= min(GHM_TOP_MAX, logits.shape[-1]):
         raise ValueError(f"top_k: 0 .. min({GHM_TOP_MAX}, V = {logits.shape[-1]}), got {top_k!r}")
+    y, bits = (None, 64) if targets is None else _ids(targets, logits.shape[:-1], logits.device, "targets")
     if torch.is_grad_enabled() and logits.requires_grad:
-        if targets is not None:
-            _ids(targets, logits.shape[:-1], logits.device, "targets")
-        return TokenScores(*_ScoreFn.apply(logits, targets, top_k, ignore_index))
-    return TokenScores(*_score(logits, targets, top_k, ignore_index, False)[:4])
+        return TokenScores(*_ScoreFn.apply(logits, y, bits, top_k, ignore_index))
+    return TokenScores(*_score(logits, y, bits, top_k, ignore_index, False)[:4])
 
 
 # ---- distillation ---------------------------------------------------------
 
 
-def _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index):
-    """Checked arguments of ghm_distill / ghm_distill_bwd up to alpha, and what they keep alive."""
-    code = _check_logits(logits)
-    dev, lead, V = logits.device, logits.shape[:-1], logits.shape[-1]
+def _distill_check(logits, top_ids, top_logits, targets, temperature, alpha):
+    """Checked arguments: (logits, ids, t, y) and (id bits, target bits, temperature, alpha)."""
+    _check_logits(logits)
+    dev, lead = logits.device, logits.shape[:-1]
     k = top_ids.shape[-1] if isinstance(top_ids, torch.Tensor) and top_ids.dim() else 0
     if not 1 <= k <= GHM_DISTILL_MAX:
         raise ValueError(f"top_ids: expected [..., k] with k in 1 .. {GHM_DISTILL_MAX}")
     ids, ibits = _ids(top_ids, (*lead, k), dev, "top_ids", bits=(32, 64))
     if not isinstance(top_logits, torch.Tensor) or top_logits.shape != ids.shape or top_logits.device != dev:
         raise ValueError(f"top_logits: expected shape {tuple(ids.shape)} on {dev}")
-    tcode = _dtype(top_logits, "top_logits")
-    t = top_logits.detach().contiguous()
+    _dtype(top_logits, "top_logits")
     y, ybits = (None, 64) if targets is None else _ids(targets, lead, dev, "targets")
     temperature, alpha = float(temperature), float(alpha)
     if not 0 < temperature < float("inf"):
         raise ValueError(f"temperature: a finite number above 0, got {temperature}")
     if not 0 <= alpha <= 1 or (alpha < 1 and targets is None):
         raise ValueError(f"alpha: 0 .. 1, below 1 only with targets, got {alpha}")
+    return (logits, ids, top_logits.detach().contiguous(), y), (ibits, ybits, temperature, alpha)
+
+
+def _distill_args(tensors, opts, ignore_index):
+    """The arguments of ghm_distill / ghm_distill_bwd up to alpha, and the logits they point to."""
+    logits, ids, t, y = tensors
+    ibits, ybits, temperature, alpha = opts
+    V = logits.shape[-1]
     z, n_inner, so, si = _rows(logits)
-    return (z.data_ptr(), code, n_inner, so, si, logits.numel() // V, V, ids.data_ptr(), ibits, t.data_ptr(), tcode,
-            k, _ptr(y), ybits, ignore_index, temperature, alpha), (z, ids, t, y)
+    return (z.data_ptr(), _DTYPE[logits.dtype], n_inner, so, si, logits.numel() // V, V, ids.data_ptr(), ibits,
+            t.data_ptr(), _DTYPE[t.dtype], ids.shape[-1], _ptr(y), ybits, ignore_index, temperature, alpha), z
 
 
 def _distill(logits, args, reduction, grad_scale=None):
@@ -215,25 +229,24 @@ def _distill(logits, args, reduction, grad_scale=None):
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, top_ids, top_logits, targets, temperature, alpha, ignore_index, reduction):
-        args, _keep = _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index)
+    def forward(ctx, logits, ids, t, y, opts, ignore_index, reduction):
+        args, _z = _distill_args((logits, ids, t, y), opts, ignore_index)
         loss, buf, _, _ = _distill(logits, args, reduction)
-        ctx.opts = (temperature, alpha, ignore_index)
-        ctx.reduction = reduction
-        ctx.save_for_backward(logits, top_ids, top_logits, targets, buf)
+        ctx.args = opts, ignore_index, reduction
+        ctx.save_for_backward(logits, ids, t, y, buf)
         return loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
-        logits, top_ids, top_logits, targets, buf = ctx.saved_tensors
-        args, _keep = _distill_args(logits, top_ids, top_logits, targets, *ctx.opts)
+        logits, ids, t, y, buf = ctx.saved_tensors
+        opts, ignore_index, reduction = ctx.args
+        args, _z = _distill_args((logits, ids, t, y), opts, ignore_index)
         g = g.contiguous()
         dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         at = buf.data_ptr()
-        _call(logits.device, "ghm_distill_bwd", *args, at, at + 16 * args[5] if ctx.reduction == "mean" else None,
-              g.data_ptr(), int(ctx.reduction == "none"), dz.data_ptr())
-        return (dz, *[None] * 7)
+        _call(logits.device, "ghm_distill_bwd", *args, at, at + 16 * args[5] if reduction == "mean" else None,
+              g.data_ptr(), int(reduction == "none"), dz.data_ptr())
+        return dz, None, None, None, None, None, None
 
 
 def _check_reduction(reduction):
@@ -259,9 +272,10 @@ def distill_loss(logits, top_ids, top_logits, targets=None, *, temperature=1.0, 
     above V, or a target outside 0 .. V - 1, makes its row NaN.  The teacher's logits get no
     gradient."""
     _check_reduction(reduction)
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        return _DistillFn.apply(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index, reduction)
-    args, _keep = _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index)
+    tensors, opts = _distill_check(logits, top_ids, top_logits, targets, temperature, alpha)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillFn.apply(*tensors, opts, ignore_index, reduction)
+    args, _z = _distill_args(tensors, opts, ignore_index)
     return _distill(logits, args, reduction)[0]
 
 
@@ -271,7 +285,8 @@ def distill_loss_and_grad(logits, top_ids, top_logits, targets=None, *, temperat
     "none": the gradient of the sum) from one call, outside autograd, as the fused
     trainers take their losses: (loss, dlogits)."""
     _check_reduction(reduction)
-    args, _keep = _distill_args(logits, top_ids, top_logits, targets, temperature, alpha, ignore_index)
+    tensors, opts = _distill_check(logits, top_ids, top_logits, targets, temperature, alpha)
+    args, _z = _distill_args(tensors, opts, ignore_index)
     loss, _, _, dz = _distill(logits, args, reduction, float(grad_scale))
     return loss, dz
 
@@ -294,40 +309,39 @@ class TopLogitsDistillLoss(nn.Module):
 # ---- embedding ------------------------------------------------------------
 
 
-def _embed(tokens, weight, scale):
-    code, dev = _DTYPE[weight.dtype], weight.device
+def _embed(tok, bits, weight, scale):
     V, D = weight.shape
-    tok, bits = _ids(tokens, tokens.shape, dev, "tokens")
     w = weight if D == 1 or weight.stride(1) == 1 else weight.contiguous()
-    out = torch.empty((*tokens.shape, D), dtype=weight.dtype, device=dev)
-    _call(dev, "ghm_embed_rows_fwd", tok.data_ptr(), bits, w.data_ptr(), code, w.stride(0), scale, out.data_ptr(),
-          tok.numel(), V, D)
+    out = torch.empty((*tok.shape, D), dtype=weight.dtype, device=weight.device)
+    _call(weight.device, "ghm_embed_rows_fwd", tok.data_ptr(), bits, w.data_ptr(), _DTYPE[weight.dtype], w.stride(0),
+          scale, out.data_ptr(), tok.numel(), V, D)
     return out
 
 
 class _EmbedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx):
-        ctx.save_for_backward(tokens)
-        ctx.shape, ctx.scale, ctx.padding_idx = weight.shape, scale, padding_idx
-        return _embed(tokens, weight, scale)
+    def forward(ctx, weight, tok, bits, scale, padding_idx):
+        ctx.save_for_backward(tok)
+        ctx.args = bits, scale, padding_idx, weight.shape
+        return _embed(tok, bits, weight, scale)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
-        tokens, = ctx.saved_tensors
-        V, D = ctx.shape
-        tok, bits = _ids(tokens, tokens.shape, g.device, "tokens")
-        g, n_inner, so, si = _rows(g)
-        N = tok.numel()
-        if n_inner != max(1, N):
-            g, si = g.contiguous(), D
-        dw = torch.empty(V, D, dtype=g.dtype, device=g.device)
+        tok, = ctx.saved_tensors
+        bits, scale, padding_idx, (V, D) = ctx.args
+        N, dev = tok.numel(), g.device
+        if g.is_contiguous():
+            stride = D
+        else:
+            g, n_inner, _, stride = _rows(g)
+            if n_inner != max(1, N):  # rows of two strides
+                g, stride = g.contiguous(), D
+        dw = torch.empty((V, D), dtype=g.dtype, device=dev)
         nws = _native.hip_lib().ghm_embed_rows_bwd_ws(N, V, D)
-        ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws else None
-        _call(g.device, "ghm_embed_rows_bwd", tok.data_ptr(), bits, g.data_ptr(), _DTYPE[g.dtype], si, ctx.scale,
-              ctx.padding_idx, dw.data_ptr(), N, V, D, _ptr(ws), nws)
-        return None, dw, None, None
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        _call(dev, "ghm_embed_rows_bwd", tok.data_ptr(), bits, g.data_ptr(), _DTYPE[g.dtype], stride, scale, padding_idx,
+              dw.data_ptr(), N, V, D, ws.data_ptr(), nws)
+        return dw, None, None, None, None
 
 
 def scaled_embedding(tokens, weight, scale=1.0, padding_idx=None):
@@ -340,10 +354,8 @@ def scaled_embedding(tokens, weight, scale=1.0, padding_idx=None):
     _dtype(weight, "weight")
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"weight: expected [V, D], got {tuple(weight.shape)}")
+    tok, bits = _ids(tokens, getattr(tokens, "shape", None), weight.device, "tokens")
     V = weight.shape[0]
-    if not isinstance(tokens, torch.Tensor):
-        raise TypeError("tokens: an integer tensor")
-    _ids(tokens, tokens.shape, weight.device, "tokens")
     if padding_idx is None:
         padding_idx = -1
     elif not -V <= padding_idx < V:
@@ -351,8 +363,8 @@ def scaled_embedding(tokens, weight, scale=1.0, padding_idx=None):
     elif padding_idx < 0:
         padding_idx += V
     if torch.is_grad_enabled() and weight.requires_grad:
-        return _EmbedFn.apply(tokens, weight, float(scale), padding_idx)
-    return _embed(tokens, weight, float(scale))
+        return _EmbedFn.apply(weight, tok, bits, float(scale), padding_idx)
+    return _embed(tok, bits, weight, float(scale))
 
 
 class ScaledEmbedding(nn.Embedding):
