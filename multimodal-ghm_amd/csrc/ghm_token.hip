@@ -165,26 +165,36 @@ __device__ __forceinline__ float group_sum(float v, float* slot, int w) {
 // The maximum starts at the lowest finite value, so differences never are -inf minus
 // -inf; a difference is cut at -1e4 where it is a factor (e^-1e4 = 0).  NaN and +inf
 // make s NaN.  c1, c2 carry log2 e.
+// EXACT: values at the maximum are counted in n and not added to the sums, so that the
+// logarithm of a sum just above 1 keeps its digits (log1p): a row with one likely value
+// of few.  Rows of up to 256 values afford the two instructions per value.
 enum { SECOND_NONE, SECOND_ENT, SECOND_EXP };
 struct Sums {
-  float m = -FLT_MAX, s = 0.f, t = 0.f;
+  float m = -FLT_MAX, s = 0.f, t = 0.f, n = 0.f;
+  __device__ __forceinline__ float total() const { return n + s; }
+  __device__ __forceinline__ float log_s() const { return n == 1.f ? log1pf(s) : logf(n + s); }
+  __device__ __forceinline__ float log_t() const { return n == 1.f ? log1pf(t) : logf(n + t); }  // SECOND_EXP
 };
 template <int SECOND>
 __device__ __forceinline__ void rebase(Sums& a, float m, float c1, float c2) {
   const float dm = fmaxf(a.m - m, -1e4f), f = __builtin_amdgcn_exp2f(dm * c1);
-  if constexpr (SECOND == SECOND_ENT) a.t = f * (a.t + dm * a.s);
-  if constexpr (SECOND == SECOND_EXP) a.t *= __builtin_amdgcn_exp2f(dm * c2);
-  a.s *= f;
+  const float n = dm == 0.f ? 0.f : a.n;  // what was at the old maximum joins the sums
+  if constexpr (SECOND == SECOND_ENT) a.t = f * (a.t + dm * (a.s + n));
+  if constexpr (SECOND == SECOND_EXP) a.t = __builtin_amdgcn_exp2f(dm * c2) * (a.t + n);
+  a.s = f * (a.s + n);
+  a.n -= n;
   a.m = m;
 }
-template <int SECOND, int N>
+template <int SECOND, bool EXACT, int N>
 __device__ __forceinline__ void fold(Sums& a, const float (&x)[N], float c1, float c2) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float d = x[i] - a.m, e = __builtin_amdgcn_exp2f(d * c1);
-    a.s += e;
+    const bool top = EXACT && d == 0.f;
+    if constexpr (EXACT) a.n += top ? 1.f : 0.f;
+    a.s += top ? 0.f : e;
     if constexpr (SECOND == SECOND_ENT) a.t += e * fmaxf(d, -1e4f);
-    if constexpr (SECOND == SECOND_EXP) a.t += __builtin_amdgcn_exp2f(d * c2);
+    if constexpr (SECOND == SECOND_EXP) a.t += top ? 0.f : __builtin_amdgcn_exp2f(d * c2);
   }
 }
 // the group's sums in every lane
@@ -193,6 +203,7 @@ __device__ __forceinline__ Sums group_join(Sums a, float* slots, int w, float c1
   rebase<SECOND>(a, group_max<W>(a.m, slots, w), c1, c2);
   a.s = wave_sum(a.s);
   if constexpr (SECOND != SECOND_NONE) a.t = wave_sum(a.t);
+  if constexpr (W == 1) a.n = wave_sum(a.n);  // EXACT rows are one wave's
   if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) {
       slots[W + w] = a.s;
@@ -320,7 +331,7 @@ __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, f
     }
     rebase<SECOND>(a, fmaxf(a.m, bm), c1, c2);
 #pragma unroll
-    for (int u = 0; u < U; ++u) fold<SECOND>(a, x[u], c1, c2);
+    for (int u = 0; u < U; ++u) fold<SECOND, N == 1>(a, x[u], c1, c2);
     if constexpr (TOP) {
       if (((b + 1) & b) == 0 || b == nb - 1) {  // the shared bound, after batches 1, 2, 4, 8, ... and the last
         const uint32_t K = kth_bits(order_bits(a.m), r);
@@ -430,11 +441,6 @@ __device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N,
   }
 }
 
-// ---------------------------------------------------------------------------
-// Scores: m = max z, s = sum e^(z - m), log p_v = (z_v - m) - log s,
-// H = log s - sum e^(z - m) (z - m) / s.  A value of -inf has probability 0 and
-// adds nothing; a row without a finite maximum has no distribution (NaN).
-// ---------------------------------------------------------------------------
 // The same by k searches of the whole range, for one that holds NaN or +inf.
 template <typename T, int N, int W, typename F>
 __device__ __forceinline__ void top_search(const T* z, int lo, int hi, TopLds<N, W>* lds, int k, int w, int lane,
@@ -463,6 +469,11 @@ __device__ __forceinline__ void top_search(const T* z, int lo, int hi, TopLds<N,
   }
 }
 
+// ---------------------------------------------------------------------------
+// Scores: m = max z, s = sum e^(z - m), log p_v = (z_v - m) - log s,
+// H = log s - sum e^(z - m) (z - m) / s.  A value of -inf has probability 0 and
+// adds nothing; a row without a finite maximum has no distribution (NaN).
+// ---------------------------------------------------------------------------
 struct ScoreOut {
   float *logprob, *entropy;
   float2* stats;
@@ -482,11 +493,10 @@ __device__ __forceinline__ void score_padding(const ScoreOut& o, int64_t r, int 
   }
 }
 // zy: the target's logit, NaN for a target outside the vocabulary
-__device__ __forceinline__ void score_write(const ScoreOut& o, int64_t r, float m, float s, float t, float zy) {
-  const float ls = logf(s);
-  if (o.logprob) o.logprob[r] = (zy - m) - ls;
-  if (o.entropy) o.entropy[r] = ls - t / s;
-  if (o.stats) o.stats[r] = make_float2(m, ls);
+__device__ __forceinline__ void score_write(const ScoreOut& o, int64_t r, const Sums& a, float ls, float zy) {
+  if (o.logprob) o.logprob[r] = (zy - a.m) - ls;
+  if (o.entropy) o.entropy[r] = ls - a.t / a.total();
+  if (o.stats) o.stats[r] = make_float2(a.m, ls);
 }
 __device__ __forceinline__ void score_top(const ScoreOut& o, int64_t r, int j, uint64_t key, float m, float ls) {
   o.top_id[r * o.top_k + j] = 0xffffffffu - static_cast<uint32_t>(key);
@@ -525,13 +535,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
   TopState top;
   Sums a = scan_row<T, N, U, W, SECOND_ENT, TOP>(z, lo, hi, LOG2E, LOG2E, w, lane, out.top_k, lds, top);
   a = group_join<SECOND_ENT, W>(a, slots, w, LOG2E, LOG2E);
+  const float ls = a.log_s();
   if (part_sums) {
     if (w == 0 && lane == 0) part_sums[item] = make_float4(a.m, a.s, a.t, 0.f);
   } else if (w == 0 && lane == 0) {
-    score_write(out, r, a.m, a.s, a.t, zy);
+    score_write(out, r, a, ls, zy);
   }
   if constexpr (TOP) {
-    const float ls = logf(a.s);
     const auto emit = [&](int j, uint64_t key) {
       if (part_sums) part_keys[item * out.top_k + j] = key;
       else score_top(out, r, j, key, a.m, ls);
@@ -567,11 +577,11 @@ __global__ __launch_bounds__(256) void k_score_join(Rows rows, int V, Ids target
   rebase<SECOND_ENT>(a, wave_max(a.m), LOG2E, LOG2E);
   a.s = wave_sum(a.s);
   a.t = wave_sum(a.t);
+  const float ls = a.log_s();
   if (threadIdx.x == 0)
-    score_write(out, r, a.m, a.s, a.t, y >= 0 && y < V ? to_f(row_ptr<T>(rows, r)[y]) : __builtin_nanf(""));
+    score_write(out, r, a, ls, y >= 0 && y < V ? to_f(row_ptr<T>(rows, r)[y]) : __builtin_nanf(""));
   const int k = out.top_k;
   if (k == 0) return;
-  const float ls = logf(a.s);
   const uint64_t* keys = part_keys + r * parts * k;
   const int q = (k + parts - 1) / parts;
   const uint32_t K = kth_bits(lane < parts ? static_cast<uint32_t>(keys[lane * k + q - 1] >> 32) : 0, (k + q - 1) / q);
@@ -611,13 +621,13 @@ __global__ __launch_bounds__(256) void k_score_short(Rows rows, int64_t n_rows, 
     x[v] = v < V ? to_f(z[v]) : NEG_INF;
     a.m = fmaxf(a.m, x[v]);
   }
-  fold<SECOND_ENT>(a, x, LOG2E, LOG2E);
+  fold<SECOND_ENT, true>(a, x, LOG2E, LOG2E);
   float zy = __builtin_nanf("");
 #pragma unroll
   for (int v = 0; v < M; ++v)
     if (v == y && v < V) zy = x[v];
-  score_write(out, r, a.m, a.s, a.t, zy);
-  const float ls = logf(a.s);
+  const float ls = a.log_s();
+  score_write(out, r, a, ls, zy);
   uint32_t left = V < 32 ? (1u << V) - 1 : 0xffffffffu;
   for (int j = 0; j < out.top_k; ++j) {
     uint64_t best = 0;
@@ -1053,7 +1063,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
   TeacherLds<W>& lds = teach[wave / W];
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
   a = group_join<SECOND, W>(a, slots, w, mix.c1, mix.c2);
-  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
   const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
   if (w == 0 && lane == 0) {
@@ -1130,11 +1140,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = i < skip ? NEG_INF : x[i];
     }
-    fold<SECOND>(a, x, mix.c1, mix.c2);
+    fold<SECOND, false>(a, x, mix.c1, mix.c2);
   }
   a.s = group_sum<W>(a.s, slots + W, w);
   if constexpr (TWO) a.t = group_sum<W>(a.t, slots + 2 * W, w);
-  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   const float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
   const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
   if (w == 0 && lane == 0) {
@@ -1204,7 +1214,7 @@ __global__ __launch_bounds__(256) void k_distill_join(Rows rows, int V, Teacher 
   a.s = wave_sum(a.s);
   if constexpr (TWO) a.t = wave_sum(a.t);
   const TeacherRow tr = teacher_row<4>(tc, r, V, mix.it, lds, w, lane);
-  const float l1 = logf(a.s), l2 = TWO ? logf(a.t) : l1;
+  const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   const float loss = distill_row_loss<T, 4>(row_ptr<T>(rows, r), V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
   if (threadIdx.x == 0) {
     row_loss[r] = tr.bad || (targets.p && (y < 0 || y >= V)) ? __builtin_nanf("") : loss;
@@ -1276,14 +1286,8 @@ __global__ __launch_bounds__(256) void k_distill_short(Rows rows, int64_t n_rows
     a.m = fmaxf(a.m, x[v]);
     q[v] = 0.f;
   }
-  float s2 = 0.f;
-#pragma unroll
-  for (int v = 0; v < M; ++v) {
-    const float d = x[v] - a.m;
-    a.s += __builtin_amdgcn_exp2f(d * LOG2E);
-    s2 += __builtin_amdgcn_exp2f(d * (mix.it * LOG2E));
-  }
-  const float l1 = logf(a.s), l2 = logf(s2);
+  fold<SECOND_EXP, true>(a, x, LOG2E, mix.c2);
+  const float l1 = a.log_s(), l2 = a.log_t();
   float st = 0.f, kl = 0.f;
   for (int j = 0; j < tc.k; ++j)
     if (teacher_has(tc, r * tc.k + j))
@@ -1851,7 +1855,7 @@ inline bool dtype_ok(int d) { return d >= 0 && d <= 2; }
 
 #define TOK_CHECK_ROWS()                                                                                       \
   GHM_CHECK(dtype_ok(dtype), "dtype (0 f32, 1 bf16, 2 f16)");                                                  \
-  GHM_CHECK(rows >= 0 && rows < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31), "shape (rows, V < 2^31)"); \
+  GHM_CHECK(rows >= 0 && rows < (int64_t(1) << 31) && V >= 1 && V <= (int64_t(1) << 30), "shape (rows < 2^31, V <= 2^30)"); \
   GHM_CHECK(n_inner >= 1 && s_outer >= 0 && s_inner >= 0, "row strides")
 
 extern "C" int64_t ghm_token_logprobs_ws(int64_t rows, int64_t V, int top_k, int dtype) {
@@ -1975,7 +1979,7 @@ extern "C" int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_i
   GHM_CHECK(ids_ok(id_bits) && id_bits != 8 && dtype_ok(t_dtype), "top_ids (32 or 64 bits), top_logits dtype"); \
   GHM_CHECK(!targets || ids_ok(target_bits), "target_bits (8, 32, 64)");                                        \
   GHM_CHECK(k >= 1 && k <= GHM_DISTILL_MAX, "k (1 .. 1024)");                                                   \
-  GHM_CHECK(temperature > 0.f && temperature <= FLT_MAX, "temperature");                                        \
+  GHM_CHECK(temperature >= 1e-6f && temperature <= 1e6f, "temperature (1e-6 .. 1e6)");                                      \
   GHM_CHECK(alpha >= 0.f && alpha <= 1.f && (targets || alpha == 1.f), "alpha (0 .. 1; below 1 needs targets)")
 
 namespace {

@@ -194,8 +194,8 @@ def _distill_check(logits, top_ids, top_logits, targets, temperature, alpha):
     _dtype(top_logits, "top_logits")
     y, ybits = (None, 64) if targets is None else _ids(targets, lead, dev, "targets")
     temperature, alpha = float(temperature), float(alpha)
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"temperature: a finite number above 0, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature: 1e-6 .. 1e6, got {temperature}")
     if not 0 <= alpha <= 1 or (alpha < 1 and targets is None):
         raise ValueError(f"alpha: 0 .. 1, below 1 only with targets, got {alpha}")
     return (logits, ids, top_logits.detach().contiguous(), y), (ibits, ybits, temperature, alpha)
