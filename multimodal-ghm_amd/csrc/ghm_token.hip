@@ -9,6 +9,7 @@
 #include "ghm_launch.h"
 
 #include <float.h>
+#include <type_traits>
 
 namespace {
 
@@ -114,15 +115,29 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
+// f over the 64 lanes, in every lane, on the vector unit alone: lane pairs, quads, eights and
+// rows of 16 by DPP, then rows 0 / 1 and 2 / 3, then the halves.  (Through the LDS crossbar
+// a distillation step of 111,848 rows of 600 values, seven of these each, took 238 us.)
+template <typename F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+  const auto dpp = [](float x, auto ctrl) {
+    const int i = __float_as_int(x);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  v = f(v, dpp(v, std::integral_constant<int, 0xb1>()));   // quad_perm 1 0 3 2
+  v = f(v, dpp(v, std::integral_constant<int, 0x4e>()));   // quad_perm 2 3 0 1
+  v = f(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
+  v = f(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return wave_all(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ void wave_fence() {  // this wave's LDS writes before its later reads
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
