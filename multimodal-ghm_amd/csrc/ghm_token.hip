@@ -933,18 +933,26 @@ __global__ __launch_bounds__(64) void k_distill_total2(const float2* __restrict_
   if (threadIdx.x == 0) distill_result(s, c, mean, loss, norm);
 }
 
-// A row's teacher in LDS: ids (-1 absent) and q; log q = (t - mt) it - lt.
+// A row's teacher in LDS: ids (-1 absent) and q; log q = (t - mt) it - lt.  The entries take
+// 8 k bytes per group of the launch's dynamic LDS (room for 1,024 of them in every block
+// halved the waves per CU of short rows), group g's after those of the groups before.
 template <int W>
 struct TeacherLds {
-  int id[GHM_DISTILL_MAX];
-  float q[GHM_DISTILL_MAX], slots[8 * W];
+  int* id;
+  float *q, *slots;
 };
+extern __shared__ float teacher_lds[];
+template <int W>
+__device__ __forceinline__ TeacherLds<W> teacher_at(int group, int k, float* slots) {
+  float* at = teacher_lds + 2 * k * group;
+  return {reinterpret_cast<int*>(at), at + k, slots};
+}
 struct TeacherRow {
   float mt, lt;
   bool some, bad;  // an entry is present; one lies outside the vocabulary
 };
 template <int W>
-__device__ __forceinline__ TeacherRow teacher_row(const Teacher& t, int64_t r, int V, float it, TeacherLds<W>& lds,
+__device__ __forceinline__ TeacherRow teacher_row(const Teacher& t, int64_t r, int V, float it, const TeacherLds<W>& lds,
                                                   int w, int lane) {
   TeacherRow o;
   float mt = -FLT_MAX, bad = 0.f;
@@ -973,7 +981,7 @@ __device__ __forceinline__ TeacherRow teacher_row(const Teacher& t, int64_t r, i
 // the loss of a row from its sums and its teacher; y checked by the caller's group
 template <typename T, int W>
 __device__ __forceinline__ float distill_row_loss(const T* z, int V, const Teacher& tc, int64_t r, const Mix& mix,
-                                                  const TeacherRow& tr, TeacherLds<W>& lds, float m, float l1, float l2,
+                                                  const TeacherRow& tr, const TeacherLds<W>& lds, float m, float l1, float l2,
                                                   int64_t y, int w, int lane) {
   float kl = 0.f;
   for (int j = w * 64 + lane; j < tc.k; j += W * 64) {
@@ -1057,7 +1065,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
                                                                    T* __restrict__ dz) {
   constexpr int G = W == 1 ? 4 : 1, SECOND = TWO ? SECOND_EXP : SECOND_NONE;
   __shared__ float slots[3 * W];
-  __shared__ TeacherLds<W> teach[G];
+  __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
   if (r >= n_rows) return;
@@ -1075,7 +1083,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
   TopState no;
   Sums a = scan_row<T, N, U, W, SECOND, false>(z, 0, V, mix.c1, mix.c2, w, lane, 0,
                                                static_cast<TopLds<N, W>*>(nullptr), no);
-  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherLds<W> lds = teacher_at<W>(wave / W, tc.k, teach_slots[wave / W]);
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
   a = group_join<SECOND, W>(a, slots, w, mix.c1, mix.c2);
   const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
@@ -1109,7 +1117,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
                                                                         T* __restrict__ dz) {
   constexpr int G = W == 1 ? 4 : 1, N = Vec<T>::N, SECOND = TWO ? SECOND_EXP : SECOND_NONE;
   __shared__ float slots[3 * W];
-  __shared__ TeacherLds<W> teach[G];
+  __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
   if (r >= n_rows) return;
@@ -1132,7 +1140,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
     const int v = v0 + u * W * 64, at = v < nv ? v * N : V - N;
     raw[u] = *reinterpret_cast<const typename Vec<T>::raw*>(z + (at + N <= V ? at : V - N));
   }
-  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherLds<W> lds = teacher_at<W>(wave / W, tc.k, teach_slots[wave / W]);
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
   Sums a;
 #pragma unroll
@@ -1209,7 +1217,8 @@ __global__ __launch_bounds__(256) void k_distill_join(Rows rows, int V, Teacher 
                                                       Mix mix, int parts, const float4* __restrict__ part_sums,
                                                       float* __restrict__ row_loss, float4* __restrict__ row_stats) {
   constexpr int SECOND = TWO ? SECOND_EXP : SECOND_NONE;
-  __shared__ TeacherLds<4> lds;
+  __shared__ float teach_slots[16];
+  const TeacherLds<4> lds = teacher_at<4>(0, tc.k, teach_slots);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t r = blockIdx.x;
   if (!row_counts(tc, targets, ignore, r, lane)) {
@@ -1242,7 +1251,7 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
                                                       int64_t ignore, Mix mix, Upstream up, int parts, int part_len,
                                                       const float4* __restrict__ row_stats, T* __restrict__ dz) {
   constexpr int G = 4 / W;
-  __shared__ TeacherLds<W> teach[G];
+  __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W, r = item / parts;
   if (r >= n_rows) return;
@@ -1254,7 +1263,7 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
     return;
   }
   const int64_t y = targets.p ? ld_id(targets, r) : -1;
-  TeacherLds<W>& lds = teach[wave / W];
+  const TeacherLds<W> lds = teacher_at<W>(wave / W, tc.k, teach_slots[wave / W]);
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
   const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
   distill_row_grad<T, N, U, W>(
@@ -2030,10 +2039,10 @@ void launch_distill(const Distill& a, const Upstream& up, T* dz) {
   constexpr int G = W == 1 ? 4 : 1;
   const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
   if (a.mix.two)
-    hipLaunchKernelGGL((k_distill<T, N, U, W, true>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+    hipLaunchKernelGGL((k_distill<T, N, U, W, true>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
   else
-    hipLaunchKernelGGL((k_distill<T, N, U, W, false>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+    hipLaunchKernelGGL((k_distill<T, N, U, W, false>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
 }
 template <typename T, int R, int W>
@@ -2041,17 +2050,17 @@ void launch_step(const Distill& a, const Upstream& up, T* dz) {
   constexpr int G = W == 1 ? 4 : 1;
   const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
   if (a.mix.two)
-    hipLaunchKernelGGL((k_distill_step<T, R, W, true>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+    hipLaunchKernelGGL((k_distill_step<T, R, W, true>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
   else
-    hipLaunchKernelGGL((k_distill_step<T, R, W, false>), g, b, 0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
+    hipLaunchKernelGGL((k_distill_step<T, R, W, false>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
 }
 template <typename T, int N, int U, int W>
 void launch_distill_grad(const Distill& a, const Upstream& up, const Split& p, T* dz) {
   constexpr int G = 4 / W;
   hipLaunchKernelGGL((k_distill_grad<T, N, U, W>), dim3(static_cast<unsigned>((a.rows * p.parts + G - 1) / G)), dim3(256),
-                     0, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up, p.parts, p.len, a.stats, dz);
+                     8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up, p.parts, p.len, a.stats, dz);
 }
 template <typename T>
 void distill_short(const Distill& a, const Upstream& up, float* row_loss, T* dz) {
@@ -2105,12 +2114,12 @@ void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) 
     if (a.mix.two) {
       hipLaunchKernelGGL((k_distill_part<T, N, 4, 8, true>), g, dim3(512), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix,
                          p.parts, p.len, sums);
-      hipLaunchKernelGGL((k_distill_join<T, true>), g1, dim3(256), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
+      hipLaunchKernelGGL((k_distill_join<T, true>), g1, dim3(256), 8 * a.tc.k, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
                          sums, a.row_loss, a.stats);
     } else {
       hipLaunchKernelGGL((k_distill_part<T, N, 4, 8, false>), g, dim3(512), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix,
                          p.parts, p.len, sums);
-      hipLaunchKernelGGL((k_distill_join<T, false>), g1, dim3(256), 0, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
+      hipLaunchKernelGGL((k_distill_join<T, false>), g1, dim3(256), 8 * a.tc.k, a.s, a.m, a.V, a.tc, a.t, a.ignore, a.mix, p.parts,
                          sums, a.row_loss, a.stats);
     }
     if (dz) distill_grad_any<T>(a, up, dz);
