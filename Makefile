@@ -6,8 +6,8 @@ CXX ?= g++
 LIBDIR := multimodal-ghm_amd/ghmclip/_lib
 SRC := multimodal-ghm_amd/csrc
 HIPOBJFLAGS := --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-result
-HIP_SRCS := $(SRC)/ghm_genc.hip $(SRC)/ghm_fwd.hip $(SRC)/ghm_bwd.hip $(SRC)/ghm_x3.hip $(SRC)/ghm_guide.hip $(SRC)/ghm_cdm.hip $(SRC)/ghm_vlm.hip $(SRC)/ghm_gemm.hip $(SRC)/ghm_vlm_x3.hip $(SRC)/ghm_wgrad.hip $(SRC)/ghm_optim.hip $(SRC)/ghm_eval.hip $(SRC)/ghm_token.hip
-HIP_HDRS := $(SRC)/ghm_common.h $(SRC)/ghm_launch.h $(SRC)/ghm_split.h $(SRC)/ghm_ln.h include/ghm_hip.h
+HIP_SRCS := $(SRC)/ghm_genc.hip $(SRC)/ghm_fwd.hip $(SRC)/ghm_bwd.hip $(SRC)/ghm_x3.hip $(SRC)/ghm_guide.hip $(SRC)/ghm_cdm.hip $(SRC)/ghm_vlm.hip $(SRC)/ghm_gemm.hip $(SRC)/ghm_vlm_x3.hip $(SRC)/ghm_wgrad.hip $(SRC)/ghm_optim.hip $(SRC)/ghm_eval.hip $(SRC)/ghm_score.hip $(SRC)/ghm_distill.hip $(SRC)/ghm_embed.hip
+HIP_HDRS := $(SRC)/ghm_common.h $(SRC)/ghm_launch.h $(SRC)/ghm_split.h $(SRC)/ghm_ln.h $(SRC)/ghm_token.h include/ghm_hip.h
 
 all: $(LIBDIR)/libghm_hip.so $(LIBDIR)/libghm_host.so
 
@@ -27,7 +27,7 @@ $(OBJDIR)/%.o: $(SRC)/%.hip $(HIP_HDRS)
 	$(HIPCC) $(HIPOBJFLAGS) -c -o $@ $<
 
 # no packed f32 instructions in the token operators (the host pass does not know the feature)
-$(OBJDIR)/ghm_token.o: HIPOBJFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
+$(OBJDIR)/ghm_score.o $(OBJDIR)/ghm_distill.o $(OBJDIR)/ghm_embed.o: HIPOBJFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 
 $(OBJDIR)/ghm_build_id.o: $(BUILD_ID_SRC)
 	$(CXX) -O2 -fPIC -c -o $@ $<

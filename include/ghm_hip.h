@@ -616,7 +616,8 @@ int ghm_tok_readout_bwd(const float* Z, const float* d_emb, const float* w_out, 
 int ghm_zsc_logits(const float* i_emb, int64_t n_rows, const float* t_emb, int D, const int32_t* proto_idx,
                    int n_class, int n_proto, const int32_t* n_list, int n_j, float* logits, void* stream);
 
-/* ---- token operators over a vocabulary of any size (csrc/ghm_token.hip) ---
+/* ---- token operators over a vocabulary of any size (csrc/ghm_score.hip,
+ * ghm_distill.hip, ghm_embed.hip) ---
  * The large-vocabulary counterparts of ghm_ce_kl, ghm_tok_embed_fwd and ghm_wcolsum;
  * the reference's vocabulary has 10 values and it has no counterpart of these.
  *

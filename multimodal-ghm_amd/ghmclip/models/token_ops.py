@@ -1,4 +1,4 @@
-"""Token operators over a vocabulary of any size (csrc/ghm_token.hip): scores of
+"""Token operators over a vocabulary of any size (csrc/ghm_score.hip, ghm_distill.hip, ghm_embed.hip): scores of
 given tokens, distillation from a teacher's top logits, scaled embedding.
 
 They stand beside the fixed-vocabulary kernels of the VLM (``ghm_ce_kl``,

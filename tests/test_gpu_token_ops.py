@@ -1,4 +1,4 @@
-"""The token operators (csrc/ghm_token.hip) against their definitions in 64 bits
+"""The token operators (csrc/ghm_score.hip, ghm_distill.hip, ghm_embed.hip) against their definitions in 64 bits
 (oracle/token_oracle.py, which also gives the bound that a 32-bit evaluation with one
 final rounding may be off; the values below are never measured ones)."""
 import math
