@@ -1,4 +1,4 @@
-"""Token operators in 64 bits on the CPU, from their definitions, with bounds on what
+"""Token operators in 64 bits, from their definitions, with bounds on what
 a 32-bit evaluation may be off (half a step of f32 is 2^-24 relative).
 
 Bounds, u = 2^-24: with d = z - m a term e^d carries |d| 3u (difference, product with
@@ -63,7 +63,7 @@ def score(z, targets, top_k, ignore_index=-100):
     finite_p = torch.where(p > 0, p * logp, torch.where(torch.isnan(p), p, 0.0))
     ent = -finite_p.sum(-1, keepdim=True)
     bent = bls + ed * (2 * bls + 8 * U * (1 + _chain(V))) + 4 * U * (ls.abs() + ed)
-    live = torch.ones(n, 1, dtype=torch.bool) if targets is None else (targets != ignore_index)[:, None]
+    live = torch.ones(n, 1, dtype=torch.bool, device=z.device) if targets is None else (targets != ignore_index)[:, None]
     out = {"logp": logp, "blogp": blogp, "p": p, "live": live}
     out["entropy"], out["bentropy"] = (torch.where(live, x, 0.0)[:, 0] for x in (ent, bent))
     if targets is not None:
@@ -80,7 +80,7 @@ def score(z, targets, top_k, ignore_index=-100):
 def score_grad(z, targets, r, g_lp=None, g_ent=None, g_top=None):
     """dz and its bound before the rounding to the logits' type."""
     n, V = z.shape
-    zero = torch.zeros(n, dtype=z.dtype)
+    zero = torch.zeros(n, dtype=z.dtype, device=z.device)
     g1 = zero if g_lp is None else g_lp
     g2 = (zero if g_ent is None else g_ent)[:, None]
     gs = g1[:, None] + (0 if g_top is None else g_top.sum(-1, keepdim=True))

@@ -28,7 +28,7 @@ def _M():
 
 
 def _near(got, want, bound, what):
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(want.device)
     assert got.shape == want.shape, (what, got.shape, want.shape)
     fin = torch.isfinite(want)
     assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in other places"
@@ -158,7 +158,7 @@ def test_score_targets(V, bits):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [10, 200, 3000, 9000])
+@pytest.mark.parametrize("V", [10, 40, 200, 3000, 9000, 70001])
 def test_score_masks_and_special_values(V, dtype):
     M = _M()
     z, y = _logits(10, V, dtype, V), torch.zeros(10, dtype=torch.long)
@@ -199,6 +199,60 @@ def test_score_ties(V, dtype):
         got = M.token_logprobs(z.to(DEV), top_k=k)
         assert got.logprob is None
         _check_score(z, None, k, got, f"ties k {k}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", [(1030, 3000), (1100, 9001), (520, 20001), (513, 40001), (512, 70003), (600, 131072)])
+def test_many_rows(rows, V, dtype):
+    """The kernels of many long rows (one wave or several per row, rows kept in registers or
+    read twice), checked on the device in 64 bits; vocabulary-sized offsets in odd rows."""
+    M = _M()
+    z, y = _logits(rows, V, dtype, V).to(DEV), _targets(rows, V, V).to(DEV)
+    k = 24
+    leaf = z.clone().requires_grad_()
+    got = M.token_logprobs(leaf, y, top_k=k)
+    r = O.score(z.double(), y, k)
+    for name in ("logprob", "entropy", "top_logprob"):
+        _near(getattr(got, name), r[name], r["b" + name], name)
+    assert torch.equal(got.top_id, r["top_id"])
+    none = M.token_logprobs(z, y)
+    assert none.top_id is None and none.top_logprob is None
+    _near(none.logprob, r["logprob"], r["blogprob"], "without alternatives")
+    g = torch.linspace(-1, 1, rows, device=DEV)
+    dz, = torch.autograd.grad((got.logprob, got.entropy), leaf, (g, 2 * g))
+    want, bound = O.score_grad(z.double(), y, r, g.double(), 2 * g.double())
+    _grad_near(dz, want, bound, dtype, "score gradient")
+    del r, want, bound, dz
+    ids, t = (x.to(DEV) for x in _teacher(rows, V, k, V))
+    for tau, alpha in ((1.0, 1.0), (2.0, 0.5)):
+        o = O.distill(z.double(), ids, t.double(), y if alpha < 1 else None, tau, alpha)
+        n = int(o["counted"].sum())
+        loss, dz = M.distill_loss_and_grad(z, ids, t, y if alpha < 1 else None, temperature=tau, alpha=alpha)
+        total = o["row_loss"].sum()
+        _near(loss, total / n, (o["brow_loss"].sum() + (rows + 28) * O.U * o["row_loss"].abs().sum()) / n, "mean")
+        _grad_near(dz, o["dz"] / n, (o["bdz"] + 4 * O.U * o["dz"].abs()) / n, dtype, "step")
+        loss = M.distill_loss(leaf, ids, t, y if alpha < 1 else None, temperature=tau, alpha=alpha, reduction="sum")
+        got, = torch.autograd.grad(loss, leaf)
+        _grad_near(got, o["dz"], o["bdz"] + 4 * O.U * o["dz"].abs(), dtype, "autograd")
+
+
+@pytest.mark.parametrize("V", [2, 10, 32, 33, 64, 100, 256])
+def test_likely_values_keep_their_digits(V):
+    """One value holds nearly everything: log p = -log1p(rest), relative to itself.  The rest
+    is a sum of V terms of |d| <= 24 units (3 u |d| + 2 u each), so off by (V + 90) u."""
+    M = _M()
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(40, V, generator=g)
+    y = torch.randint(0, V, (40,), generator=g)
+    z[torch.arange(40), y] += 8 + 10 * torch.rand(40, generator=g)
+    got = M.token_logprobs(z.to(DEV), y.to(DEV), top_k=1)
+    d = z.double() - z.double().gather(-1, y[:, None])
+    rest = torch.where(torch.arange(V) == y[:, None], 0.0, d.exp()).sum(-1)
+    want = -torch.log1p(rest)
+    _near(got.logprob, want, (V + 90) * O.U * want.abs(), "logprob")
+    _near(got.top_logprob[:, 0], want, (V + 90) * O.U * want.abs(), "alternative")
+    loss = M.distill_loss(z.to(DEV), y[:, None].to(DEV), torch.zeros(40, 1, device=DEV), reduction="none")
+    _near(loss, -want, (V + 94) * O.U * want.abs(), "distillation of one entry")
 
 
 def test_score_views():
@@ -491,7 +545,8 @@ def test_refusals():
     with pytest.raises(ValueError, match="V >= 1"):
         M.token_logprobs(z[:, :0])
     ids, t = torch.zeros(4, 2, dtype=torch.long, device=DEV), torch.zeros(4, 2, device=DEV)
-    for bad in (dict(temperature=0.0), dict(temperature=math.inf), dict(temperature=math.nan), dict(alpha=0.5),
+    for bad in (dict(temperature=0.0), dict(temperature=math.inf), dict(temperature=math.nan),
+                dict(temperature=1e-7), dict(temperature=1e7), dict(alpha=0.5),
                 dict(alpha=-0.1), dict(alpha=1.1), dict(reduction="median")):
         with pytest.raises(ValueError):
             M.distill_loss(z, ids, t, **bad)

@@ -25,7 +25,7 @@ def _score(**kw):
     return _lib().ghm_token_logprobs(*a.values())
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(V=0), dict(V=1 << 31), dict(rows=-1),
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(V=0), dict(V=(1 << 30) + 1), dict(rows=-1),
                                 dict(rows=1 << 31), dict(n_inner=0), dict(so=-1), dict(si=-1), dict(top_k=-1),
                                 dict(top_k=65, V=100), dict(top_k=11), dict(bits=16), dict(logits=None),
                                 dict(logprob=None), dict(targets=None), dict(top_lp=None), dict(top_id=None),
@@ -61,7 +61,7 @@ def _distill(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=3), dict(ibits=8), dict(tdtype=5), dict(k=0), dict(k=1025), dict(tau=0.0),
-                                dict(tau=-1.0), dict(tau=math.inf), dict(tau=math.nan), dict(alpha=1.5),
+                                dict(tau=-1.0), dict(tau=math.inf), dict(tau=math.nan), dict(tau=1e-7), dict(tau=1e7), dict(alpha=1.5),
                                 dict(alpha=math.nan), dict(alpha=0.5, y=None), dict(reduction=3), dict(loss=None),
                                 dict(norm=None), dict(row_loss=None), dict(stats=None), dict(logits=None),
                                 dict(ids=None), dict(t=None), dict(ybits=3), dict(ws_bytes=-1)])
@@ -94,7 +94,8 @@ def _embed_bwd(**kw):
     return _lib().ghm_embed_rows_bwd(*a.values())
 
 
-@pytest.mark.parametrize("kw", [dict(bits=9), dict(dtype=3), dict(V=0), dict(D=0), dict(N=-1), dict(tok=None)])
+@pytest.mark.parametrize("kw", [dict(bits=9), dict(dtype=3), dict(V=0), dict(V=1 << 31), dict(D=0), dict(D=(1 << 20) + 1),
+                                dict(N=-1), dict(N=1 << 31), dict(tok=None)])
 def test_embed_refusals(kw):
     assert _embed(**kw) == -22
     assert _embed_bwd(**kw) == -22
