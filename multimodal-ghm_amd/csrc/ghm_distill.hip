@@ -636,7 +636,7 @@ template <typename T>
 void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) {
   constexpr int N = Vec<T>::N;
   T* dz = static_cast<T*>(dlogits);
-  const Split p = row_split(a.rows, a.V);
+  const Split p = row_split(a.rows, a.V, N, dz ? SPLIT_STEP : SPLIT_SUMS);
   const int nv = (a.V + N - 1) / N;
   if (a.V <= SHORT_V) {
     distill_short<T>(a, up, a.row_loss, dz);
@@ -680,9 +680,8 @@ void distill_any(const Distill& a, const Upstream& up, void* dlogits, void* ws) 
 }  // namespace
 
 extern "C" int64_t ghm_distill_ws(int64_t rows, int64_t V, int dtype) {
-  (void)dtype;
   if (rows <= 0 || V <= 0) return DISTILL_WS_HEAD;
-  const Split p = row_split(rows, V);
+  const Split p = row_split(rows, V, dtype == 0 ? 4 : 8, {SPLIT_STEP.vectors, SPLIT_SUMS.rows});  // either rule's
   return DISTILL_WS_HEAD + (p.parts == 1 ? 0 : rows * p.parts * 16);
 }
 

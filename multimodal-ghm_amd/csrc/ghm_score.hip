@@ -369,9 +369,8 @@ __global__ __launch_bounds__(256) void k_score_bwd_short(Rows rows, int64_t n_ro
 }  // namespace
 
 extern "C" int64_t ghm_token_logprobs_ws(int64_t rows, int64_t V, int top_k, int dtype) {
-  (void)dtype;
   if (rows <= 0 || V <= 0 || top_k < 0) return 0;
-  const Split p = row_split(rows, V);
+  const Split p = row_split(rows, V, dtype == 0 ? 4 : 8, top_k ? SPLIT_TOP : SPLIT_SUMS);
   return p.parts == 1 ? 0 : rows * p.parts * (16 + 8 * static_cast<int64_t>(top_k));
 }
 
@@ -394,8 +393,8 @@ void launch_score(const Rows& m, int64_t rows, int V, const Ids& t, int64_t igno
 template <typename T>
 void score_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreOut& o, void* ws,
                hipStream_t s) {
-  const Split p = row_split(rows, V);
   constexpr int N = Vec<T>::N;
+  const Split p = row_split(rows, V, N, o.top_k ? SPLIT_TOP : SPLIT_SUMS);
   if (V <= SHORT_V) {
     const dim3 g(static_cast<unsigned>((rows + 255) / 256));
     if (V <= 12) hipLaunchKernelGGL((k_score_short<T, 12>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);

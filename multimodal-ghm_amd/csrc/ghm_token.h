@@ -384,21 +384,31 @@ __device__ __forceinline__ Sums scan_row(const T* z, int lo, int hi, float c1, f
 
 constexpr int SHORT_V = 32;  // rows of at most this many values: one lane per row
 
-// How a row is split (both kinds of logits operator): rows few and long go in parts so
-// that about 512 groups are at work, each with at least one vector per lane of 8 waves.
+// Rows of up to 256 vectors take one wave, up to 1,536 too where there are many of them
+// (scores of 16,777 rows of 4,000 bf16 values: 30 us by one wave, 34 by two, 56 by four).
+inline bool one_wave(int64_t rows, int64_t V, int N) {
+  return V <= 256 * N || (V <= 1536 * N && rows >= 1024);
+}
+
+// Few, long rows go in parts of at least 4,096 values, about 512 in all, and a second launch
+// joins a row's parts: only where that pays for the launch (4 rows of 131,072 bf16 values
+// with 20 alternatives: 12 us in parts, 18 whole; of 32,000 values: 11 and 9.5).  The
+// callers' thresholds, in vectors and rows:
 constexpr int MAX_PARTS = 64;  // of a row
 struct Split {
   int parts, len;
 };
-inline bool one_wave(int64_t rows, int64_t V, int N) {
-  return V <= 256 * N || (V <= 1536 * N && rows >= 1024);
-}
-inline Split row_split(int64_t rows, int64_t V) {
-  const int64_t most = V / 4096;
-  int64_t p = rows > 0 && rows < 512 ? (512 + rows - 1) / rows : 1;
-  if (p > most) p = most;
+struct SplitRule {
+  int64_t vectors, rows;
+};
+constexpr SplitRule SPLIT_TOP{8192, 511};   // scores with alternatives
+constexpr SplitRule SPLIT_SUMS{32768, 64};  // sums alone: 100 rows of 131,072 f32 values 15 us in parts, 14 whole
+constexpr SplitRule SPLIT_STEP{16384, 32};  // sums and gradient: 100 rows of 131,072 bf16 values 33 us in parts, 26 whole
+inline Split row_split(int64_t rows, int64_t V, int N, SplitRule rule) {
+  if (rows < 1 || rows > rule.rows || V <= rule.vectors * N) return {1, static_cast<int>(V)};
+  int64_t p = (512 + rows - 1) / rows;
+  if (p > V / 4096) p = V / 4096;
   if (p > MAX_PARTS) p = MAX_PARTS;
-  if (p < 2) return {1, static_cast<int>(V)};
   int64_t len = (V + p - 1) / p;
   len = (len + 511) / 512 * 512;
   return {static_cast<int>((V + len - 1) / len), static_cast<int>(len)};

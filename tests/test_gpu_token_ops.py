@@ -73,7 +73,7 @@ def _check_score(z, y, k, got, what, ignore=-100):
 
 SHAPES = [(1, 1), (3, 2), (5, 10), (513, 10), (7, 31), (7, 32), (7, 33), (4, 64), (3, 65), (66, 127), (2, 257), (9, 500),
           (5, 1000), (2, 1024), (2, 2048), (2, 2049), (6, 3999), (3, 4097), (2, 8193), (1, 32771), (3, 70001), (300, 513),
-          (1, 200003)]
+          (1, 200003), (5, 140001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -361,7 +361,7 @@ def test_distill(rows, V, dtype):
         _check_distill(z, ids, t, y if alpha < 1 or k == 1 else None, tau, alpha, dtype, f"k {k} tau {tau} alpha {alpha}")
 
 
-@pytest.mark.parametrize("V", [10, 40, 3000, 20000])
+@pytest.mark.parametrize("V", [10, 40, 3000, 20000, 70001])
 @pytest.mark.parametrize("k", [1, 3, 1000, 1024])
 def test_distill_entries(V, k):
     """More entries than values, repeated ids, teacher logits of 16 bits, 32-bit ids."""
@@ -380,7 +380,7 @@ def test_distill_entries(V, k):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
-@pytest.mark.parametrize("V", [10, 300, 3000, 20000])
+@pytest.mark.parametrize("V", [10, 300, 3000, 20000, 70001])
 def test_distill_special_values(V):
     M = _M()
     z = _logits(8, V, torch.float32, V)
