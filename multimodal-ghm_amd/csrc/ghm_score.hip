@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256) void k_score_join(Rows rows, int V, Ids target
 // Rows of at most SHORT_V values: one lane per row, the row in registers, the
 // alternatives by k searches.
 template <typename T, int M>
-__global__ __launch_bounds__(256) void k_score_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
-                                                     ScoreOut out) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__global__ __launch_bounds__(64) void k_score_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
+                                                    ScoreOut out) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
   if (r >= n_rows) return;
   const int64_t y = targets.p ? ld_id(targets, r) : 0;
   if (targets.p && y == ignore) {
@@ -333,9 +333,9 @@ __global__ __launch_bounds__(256) void k_score_bwd(Rows rows, int64_t n_rows, in
 }
 
 template <typename T, int M>
-__global__ __launch_bounds__(256) void k_score_bwd_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
-                                                         ScoreGrad g, T* __restrict__ dz) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__global__ __launch_bounds__(64) void k_score_bwd_short(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
+                                                        ScoreGrad g, T* __restrict__ dz) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
   if (r >= n_rows) return;
   T* d = dz + r * V;
   const int64_t y = targets.p ? ld_id(targets, r) : -1;
@@ -396,9 +396,9 @@ void score_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore,
   constexpr int N = Vec<T>::N;
   const Split p = row_split(rows, V, N, o.top_k ? SPLIT_TOP : SPLIT_SUMS);
   if (V <= SHORT_V) {
-    const dim3 g(static_cast<unsigned>((rows + 255) / 256));
-    if (V <= 12) hipLaunchKernelGGL((k_score_short<T, 12>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
-    else hipLaunchKernelGGL((k_score_short<T, SHORT_V>), g, dim3(256), 0, s, m, rows, V, t, ignore, o);
+    const dim3 g(static_cast<unsigned>((rows + 63) / 64));
+    if (V <= 12) hipLaunchKernelGGL((k_score_short<T, 12>), g, dim3(64), 0, s, m, rows, V, t, ignore, o);
+    else hipLaunchKernelGGL((k_score_short<T, SHORT_V>), g, dim3(64), 0, s, m, rows, V, t, ignore, o);
   } else if (V <= 64) {
     launch_score<T, 1, 1, 1>(m, rows, V, t, ignore, o, p, ws, s);
   } else if (V <= 256) {
@@ -452,9 +452,9 @@ void score_bwd_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ign
   T* dz = static_cast<T*>(dlogits);
   const Split p = map_split(rows, V);
   if (V <= SHORT_V) {
-    const dim3 gr(static_cast<unsigned>((rows + 255) / 256));
-    if (V <= 12) hipLaunchKernelGGL((k_score_bwd_short<T, 12>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
-    else hipLaunchKernelGGL((k_score_bwd_short<T, SHORT_V>), gr, dim3(256), 0, s, m, rows, V, t, ignore, g, dz);
+    const dim3 gr(static_cast<unsigned>((rows + 63) / 64));
+    if (V <= 12) hipLaunchKernelGGL((k_score_bwd_short<T, 12>), gr, dim3(64), 0, s, m, rows, V, t, ignore, g, dz);
+    else hipLaunchKernelGGL((k_score_bwd_short<T, SHORT_V>), gr, dim3(64), 0, s, m, rows, V, t, ignore, g, dz);
   } else if (V <= 256) {
     launch_score_bwd<T, 1, 4, 1>(m, rows, V, t, ignore, g, p, dz, s);
   } else if (p.parts == 1 && one_wave(rows, V, N)) {
