@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
 // summed in f32, a token that crosses chunks through partial rows joined in order; table
 // rows without a token are written 0 beside it.  No atomics on values: a fixed order.
 // ---------------------------------------------------------------------------
-constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_ROUNDS = 8;
+constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_ROUNDS = 4;
 constexpr int SORT_SELF_N = 16384;  // up to this many positions a block counts them all itself
 constexpr int SORT_TILES = 128;     // up to this many tiles it sums their counts itself
 
@@ -579,7 +579,7 @@ inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
     p.key[i] = at, at += up256(N * 4);
     p.pos[i] = at, at += up256(N * 4);
   }
-  p.counts = at, at += up256((N / (64 * 4 * SORT_ROUNDS) + 2) * SORT_BINS * 4);
+  p.counts = at, at += up256((N / (64 * 8 * SORT_ROUNDS) + 2) * SORT_BINS * 4);
   p.used = at, at += up256(p.used_words * 4);
   p.parts = at, at += up256(p.chunks * 2 * D * 4);
   p.bytes = at;
@@ -626,8 +626,8 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
                        reinterpret_cast<uint32_t*>(ws + p.used), static_cast<int>(p.used_words));
   } else if (N <= SORT_SELF_N) {
     launch_sort<8, SORT_SELF>(p, tok, pad, N, V, ws, s);
-  } else if (N <= 64 * 4 * SORT_ROUNDS * SORT_TILES) {
-    launch_sort<4, SORT_SUM>(p, tok, pad, N, V, ws, s);
+  } else if (N <= 64 * 8 * SORT_ROUNDS * SORT_TILES) {
+    launch_sort<8, SORT_SUM>(p, tok, pad, N, V, ws, s);
   } else {
     launch_sort<16, SORT_SCANNED>(p, tok, pad, N, V, ws, s);
   }
