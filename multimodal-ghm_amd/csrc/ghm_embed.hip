@@ -509,6 +509,70 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
              (((red[0][i][lane] + red[1][i][lane]) + red[2][i][lane]) + red[3][i][lane]) * scale);
 }
 
+// Tables of at most FEW_V rows (the model's own 10 token values) need no sort: a block keeps
+// the sums of its positions for all rows in LDS, each column one lane's, in order; the
+// blocks' sums are joined in order by a second launch, which writes every row.  10,368
+// positions of 10 x 256 f32: 17 us, by the sort (three launches) 31; 32,768 x 1024: 43 and
+// 53; where there is more to read, the LDS sums of one row at a time fall behind (131,071 x
+// 1024 bf16 into 32 rows: 160 and 81), so up to FEW_ELEMS values only.
+constexpr int FEW_V = 32, FEW_BLOCKS = 256, FEW_JOIN = 16, FEW_ELEMS = 1 << 24;
+inline bool few_rows(int64_t N, int64_t V, int64_t D) { return V <= FEW_V && N * D <= FEW_ELEMS; }
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_few(Ids tok, const T* __restrict__ dout, int64_t d_stride, int64_t pad,
+                                                   int V, int64_t N, int D, int64_t per, float* __restrict__ parts) {
+  constexpr int C = 4 / sizeof(T), U = 8;  // columns per lane: 4 bytes of a row
+  extern __shared__ float sum[];  // [V][256 C]
+  const int64_t lo = blockIdx.x * per, hi = lo + per < N ? lo + per : N;
+  const int col0 = (blockIdx.y * 256 + threadIdx.x) * C;
+  const int col = col0 + C <= D || D < C ? col0 : D - C;  // an odd last column is shared with the one before
+  if (col0 >= D) return;
+  float* mine = sum + threadIdx.x * C;
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int c = 0; c < C; ++c) mine[v * 256 * C + c] = 0.f;
+  for (int64_t i = lo; i < hi; i += U) {
+    int64_t v[U];
+    T x[U][C];
+    const auto at = [&](int u) { return i + u < hi ? i + u : hi - 1; };
+    ld_ids<U>(tok, v, at);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const T* row = dout + at(u) * d_stride + col;
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[u][c] = row[col + c < D ? c : 0];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= hi || v[u] < 0 || v[u] >= V || v[u] == pad) continue;
+#pragma unroll
+      for (int c = 0; c < C; ++c) mine[v[u] * 256 * C + c] += to_f(x[u][c]);
+    }
+  }
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (col + c < D) parts[(static_cast<int64_t>(blockIdx.x) * V + v) * D + col + c] = mine[v * 256 * C + c];
+}
+// row v = blockIdx.x, 64 columns per block: FEW_JOIN waves take the blocks' sums in turn
+template <typename T>
+__global__ __launch_bounds__(64 * FEW_JOIN) void k_embed_few_join(const float* __restrict__ parts, int blocks, int V, int D,
+                                                                  float scale, T* __restrict__ dw) {
+  __shared__ float red[FEW_JOIN][64];
+  const int v = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.y * 64 + lane;
+  const int per = (blocks + FEW_JOIN - 1) / FEW_JOIN, a = w * per, b = a + per < blocks ? a + per : blocks;
+  float s = 0.f;
+  if (col < D) {
+#pragma unroll 16
+    for (int j = a; j < b; ++j) s += parts[(static_cast<int64_t>(j) * V + v) * D + col];
+  }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || col >= D) return;
+#pragma unroll
+  for (int j = 1; j < FEW_JOIN; ++j) s += red[j][lane];
+  from_f(dw[static_cast<int64_t>(v) * D + col], s * scale);
+}
+
 // no token at all: every table row is 0
 template <typename T>
 __global__ __launch_bounds__(256) void k_embed_zero(T* __restrict__ dw, int64_t n) {
@@ -586,6 +650,12 @@ inline EmbedPlan embed_plan(int64_t N, int64_t V, int64_t D, int ve) {
   return p;
 }
 
+// blocks of k_embed_few: 32 positions each at least; the last one is not empty
+inline int few_blocks(int64_t N) {
+  const int64_t b = (N + 31) / 32 < FEW_BLOCKS ? (N + 31) / 32 : FEW_BLOCKS, per = (N + b - 1) / b;
+  return static_cast<int>((N + per - 1) / per);
+}
+
 template <int W, int MODE>
 void launch_sort(const EmbedPlan& p, const Ids& tok, int64_t pad, int64_t N, int64_t V, char* ws, hipStream_t s) {
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
@@ -615,6 +685,18 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
   if (N == 0) {
     const int64_t n = V * D, blocks = (n + 1023) / 1024;
     hipLaunchKernelGGL(k_embed_zero<T>, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, dw, n);
+    return;
+  }
+  if (few_rows(N, V, D)) {
+    const int blocks = few_blocks(N);
+    const int64_t per = (N + blocks - 1) / blocks;
+    float* sums = reinterpret_cast<float*>(ws);
+    constexpr int cols = 256 * (4 / sizeof(T));
+    hipLaunchKernelGGL(k_embed_few<T>, dim3(blocks, static_cast<unsigned>((D + cols - 1) / cols)), dim3(256),
+                       static_cast<unsigned>(V * cols * 4), s, tok,
+                       dout, d_stride, pad, static_cast<int>(V), N, D, per, sums);
+    hipLaunchKernelGGL(k_embed_few_join<T>, dim3(static_cast<unsigned>(V), static_cast<unsigned>((D + 63) / 64)),
+                       dim3(64 * FEW_JOIN), 0, s, sums, blocks, static_cast<int>(V), D, scale, dw);
     return;
   }
   const EmbedPlan p = embed_plan(N, V, D, Vec<T>::N);
@@ -656,6 +738,7 @@ void embed_bwd_any(const Ids& tok, const T* dout, int64_t d_stride, float scale,
 
 extern "C" int64_t ghm_embed_rows_bwd_ws(int64_t N, int64_t V, int64_t D) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
+  if (few_rows(N, V, D)) return up256(static_cast<int64_t>(few_blocks(N)) * V * D * 4);
   const int64_t a = embed_plan(N, V, D, 4).bytes, b = embed_plan(N, V, D, 8).bytes;
   return a > b ? a : b;
 }

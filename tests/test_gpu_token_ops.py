@@ -459,7 +459,8 @@ def test_distill_gradient_against_differences():
 EMBED_SHAPES = [(1, 1, 1), (1, 10, 256), (7, 3, 5), (64, 10, 64), (1000, 10, 33), (513, 257, 128), (4096, 50, 8),
                 (3000, 70001, 16), (9000, 300, 96), (20000, 7, 130), (40000, 1000, 40), (33, 5, 4096), (70000, 2, 8),
                 (4097, 70001, 16), (16384, 600, 8), (16385, 3001, 24), (300, 1100000, 4), (270001, 5000, 12),
-                (9000, 511, 7), (9000, 512, 3), (100, 40, 4100), (12000, 300000, 8)]
+                (9000, 511, 7), (9000, 512, 3), (100, 40, 4100), (12000, 300000, 8),
+                (40000, 7, 450), (500, 32, 1025), (100, 33, 70)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
