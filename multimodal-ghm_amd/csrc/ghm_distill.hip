@@ -250,7 +250,12 @@ __device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int h
   distill_entries<T, W>(z, d, lo, hi, tc, mix, g, lds, y, w, lane);
 }
 
-// Sums of a row, its loss, and its gradient if dz is there, by a group of W waves.
+// Sums of a row, its loss, and its gradient if dz is there, by a group of W waves.  The
+// gradient reads the row again; its stores go past the caches so that the row is still in
+// the 256 MB one: 4,096 rows of 131,072 bf16 values, 64 entries, in 495 us (4.3 TB/s of one
+// read and one write; 553 us with ordinary stores).  That needs few enough rows in flight:
+// 16 waves on a row of more than 8,192 vectors (8 waves: 524 us), 8 on shorter ones.
+// Without a gradient 189 us (5.7 TB/s).
 // row_stats: (m, log of the hard labels' sum, log of the teacher's, counted)
 template <typename T, int N, int U, int W, bool TWO>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, int64_t n_rows, int V, Teacher tc,
@@ -303,7 +308,10 @@ __device__ __forceinline__ void hold(u32x4 (&raw)[R]) {
 }
 
 // The same with the row held in registers between the sums and the gradient (R vectors per
-// lane, R * 64 * W * N values at most): the logits are read once.
+// lane, R * 64 * W * N values at most): the logits are read once.  For rows of up to 4,096
+// vectors: 4,194 rows of 16,000 bf16 values with two softmaxes 68 us (3.9 TB/s, the two
+// exponentials twice per value), read twice 82; on longer ones a CU holds too few rows to
+// load one while it computes another (131,072 values: 590 us against 495).
 template <typename T, int R, int W, bool TWO>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_distill_step(Rows rows, int64_t n_rows, int V, Teacher tc,
                                                                         Ids targets, int64_t ignore, Mix mix,

@@ -141,6 +141,12 @@ __device__ __forceinline__ void score_top(const ScoreOut& o, int64_t r, int j, u
   o.top_lp[r * o.top_k + j] = (key_value(key) - m) - ls;
 }
 
+// One pass: every value is read once, with the running maximum, the two sums and the noting
+// of vectors on the vector unit meanwhile (about 11 instructions a value, the exponential
+// counting four).  Bound by the reads: 4,096 rows of 131,072 bf16 values in 182 us (5.9 TB/s;
+// a copy of 2 GiB runs at 4.9), with the 32 most likely values 219 us; 2,000 rows of 50,001
+// f32 values 70 us (5.8 TB/s).  Four waves per row leave more rows in flight beside one that
+// ranks its alternatives (eight: 230 us); without alternatives eight are 5 % faster.
 // Groups of W waves take a row, or one of `parts` ranges of `part_len` values of it
 // (part_sums != NULL: what they found goes there for k_score_join).
 template <typename T, int N, int U, int W, bool TOP>
@@ -302,7 +308,9 @@ __device__ __forceinline__ ScoreRow score_row(const ScoreGrad& g, int64_t r, flo
   return o;
 }
 
-// the whole row part is written first, then the target's and the alternatives' entries again
+// The whole row part is written first, then the target's and the alternatives' entries again.
+// Bound by one read and one write: 2,000 rows of 50,001 f32 values in 166 us (4.8 TB/s, a
+// copy's rate).  Stores past the caches gained nothing on whole lines and cost 5 % on these.
 template <typename T, int N, int U, int W>
 __global__ __launch_bounds__(256) void k_score_bwd(Rows rows, int64_t n_rows, int V, Ids targets, int64_t ignore,
                                                    ScoreGrad g, int parts, int part_len, T* __restrict__ dz) {

@@ -573,6 +573,86 @@ def test_refusals():
             M.scaled_embedding(y, w, padding_idx=pad)
 
 
+def test_calls_without_leading_dimensions_or_targets():
+    M = _M()
+    z = _logits(1, 50, torch.float32, 1)
+    one, y = z[0].to(DEV).requires_grad_(), torch.tensor(7, device=DEV)
+    r = O.score(z.double(), torch.tensor([7]), 3)
+    got = M.token_logprobs(one, y, top_k=3)
+    assert got.logprob.shape == () and got.top_id.shape == (3,)
+    _near(got.logprob.view(1), r["logprob"], r["blogprob"], "one row")
+    loss = M.distill_loss(one, got.top_id, got.top_logprob, y, alpha=0.5, reduction="none")
+    assert loss.shape == () and torch.autograd.grad(loss, one)[0].shape == (50,)
+    # entropy alone, no targets
+    for rows, V in ((4, 10), (4, 100), (4, 3000), (4, 140001)):
+        z = _logits(rows, V, torch.float32, V)
+        leaf = z.to(DEV).requires_grad_()
+        got = M.token_logprobs(leaf)
+        assert got.logprob is None and got.top_id is None
+        r = O.score(z.double(), None, 0)
+        dz, = torch.autograd.grad(got.entropy.sum(), leaf)
+        want, bound = O.score_grad(z.double(), None, r, None, torch.ones(rows).double())
+        _grad_near(dz, want, bound, torch.float32, "entropy alone")
+    w = torch.randn(9, 6, device=DEV, requires_grad=True)
+    out = M.scaled_embedding(torch.tensor(4, device=DEV), w, 3.0)
+    assert torch.equal(out, w[4] * 3) and out.shape == (6,)
+
+
+@pytest.mark.parametrize("V", [10, 90, 900, 9000, 70001])
+def test_distill_targets_that_only_count(V):
+    """alpha = 1 with targets: they say which rows count, and no more."""
+    z, y = _logits(7, V, torch.float32, V), _targets(7, V, V)
+    ids, t = _teacher(7, V, min(V, 6), V)
+    _check_distill(z, ids, t, y, 1.5, 1.0, torch.float32, "alpha 1 with targets")
+
+
+@pytest.mark.parametrize("N,V", [(60, 20), (60, 50), (6000, 300), (6000, 2000), (40000, 2000), (300000, 40)])
+def test_embedding_of_padding_alone(N, V):
+    """No token of the table: every row of the gradient is 0, whatever the buffer held."""
+    M = _M()
+    w = torch.randn(V, 8, device=DEV, requires_grad=True)
+    tok = torch.full((N,), 3, device=DEV)
+    tok[::2] = V + 5
+    tok[1::4] = -9
+    out = M.scaled_embedding(tok, w, 1.0, padding_idx=3)
+    junk = torch.full((V, 8), math.nan, device=DEV)
+    del junk  # the gradient is likely to take this block of the allocator
+    dw, = torch.autograd.grad(out, w, torch.full_like(out, math.nan))
+    assert (dw == 0).all()
+
+
+def test_embedding_gradient_of_two_strides():
+    M = _M()
+    g = torch.Generator().manual_seed(2)
+    tok = torch.randint(0, 40, (5, 7), generator=g)
+    w, big = torch.randn(40, 12, generator=g), torch.randn(5, 9, 12, generator=g)
+    leaf = w.to(DEV).requires_grad_()
+    dw, = torch.autograd.grad(M.scaled_embedding(tok.to(DEV), leaf, 1.5), leaf, big.to(DEV)[:, 1:8])
+    want, bound = O.embed_grad(tok.reshape(-1), big[:, 1:8].reshape(35, 12).double(), 1.5, 40)
+    _grad_near(dw, want, bound, torch.float32, "two strides")
+
+
+def test_outputs_of_more_than_2_31_values():
+    """Gradients past 32-bit offsets: the last rows of a 2.2e9-value batch."""
+    M = _M()
+    rows, V = 17000, 131072
+    z = torch.empty(rows, V, dtype=torch.bfloat16, device=DEV).normal_(0, 2)
+    y = torch.randint(0, V, (rows,), device=DEV)
+    ids, t = torch.randint(0, V, (rows, 2), device=DEV), torch.randn(rows, 2, device=DEV)
+    _, dz = M.distill_loss_and_grad(z, ids, t, reduction="sum")
+    tail = slice(rows - 4, rows)
+    o = O.distill(z[tail].double(), ids[tail], t[tail].double(), None, 1.0, 1.0)
+    _grad_near(dz[tail], o["dz"], o["bdz"], torch.bfloat16, "distillation")
+    del dz
+    leaf = z.requires_grad_()
+    got = M.token_logprobs(leaf, y, top_k=2)
+    dz, = torch.autograd.grad(got.logprob.sum(), leaf)
+    r = O.score(z.detach()[tail].double(), y[tail], 2)
+    assert torch.equal(got.top_id[tail], r["top_id"])
+    want, bound = O.score_grad(z.detach()[tail].double(), y[tail], r, torch.ones(4, device=DEV).double())
+    _grad_near(dz[tail], want, bound, torch.bfloat16, "scores")
+
+
 def test_second_gradient_is_refused():
     M = _M()
     z = torch.randn(3, 9, device=DEV, requires_grad=True)
