@@ -23,6 +23,31 @@ __device__ __forceinline__ float ld_teacher(const Teacher& t, int64_t i) {
 __device__ __forceinline__ bool teacher_has(const Teacher& t, int64_t i) {
   return ld_id(t.ids, i) >= 0 && !(ld_teacher(t, i) == NEG_INF);
 }
+// 8 entries of a row for one lane, none waiting for another (one by one, 10,240 rows of 10
+// values and 4 entries took 10.5 us in place of 7.8)
+struct Entries {
+  int64_t id[8];
+  float t[8];
+  bool has[8];
+};
+__device__ __forceinline__ Entries ld_entries(const Teacher& tc, int64_t first, int j0) {
+  Entries e;
+  const auto at = [&](int u) { return first + (j0 + u < tc.k ? j0 + u : tc.k - 1); };
+  ld_ids<8>(tc.ids, e.id, at);
+  if (tc.dtype == 0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) e.t[u] = static_cast<const float*>(tc.logits)[at(u)];
+  } else if (tc.dtype == 1) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) e.t[u] = to_f(static_cast<const bf16_t*>(tc.logits)[at(u)]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) e.t[u] = to_f(static_cast<const f16_t*>(tc.logits)[at(u)]);
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u) e.has[u] = j0 + u < tc.k && e.id[u] >= 0 && !(e.t[u] == NEG_INF);
+  return e;
+}
 // rows that count: the target is not the ignored one; without targets, an alternative is
 // present.  Asked by the whole group, answered alike in every lane.
 __device__ __forceinline__ bool row_counts(const Teacher& t, const Ids& targets, int64_t ignore, int64_t r, int lane) {
@@ -69,7 +94,11 @@ __global__ __launch_bounds__(256) void k_distill_count(Teacher t, Ids targets, i
     if (targets.p) {
       in = ld_id(targets, r) != ignore;
     } else {
-      for (int j = 0; j < t.k && !in; ++j) in = teacher_has(t, r * t.k + j);
+      for (int j0 = 0; j0 < t.k && !in; j0 += 8) {
+        const Entries e = ld_entries(t, r * t.k, j0);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) in |= e.has[u];
+      }
     }
     c += in;
   }
@@ -475,31 +504,7 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
 }
 
 // Rows of at most SHORT_V values, one lane per row: loss, statistics and gradient, each
-// if asked for.  The entries are read 8 at a time, none waiting for another (one by one,
-// 10,240 rows of 10 values and 4 entries took 10.5 us).
-struct Entries {
-  int64_t id[8];
-  float t[8];
-  bool has[8];
-};
-__device__ __forceinline__ Entries ld_entries(const Teacher& tc, int64_t first, int j0) {
-  Entries e;
-  const auto at = [&](int u) { return first + (j0 + u < tc.k ? j0 + u : tc.k - 1); };
-  ld_ids<8>(tc.ids, e.id, at);
-  if (tc.dtype == 0) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) e.t[u] = static_cast<const float*>(tc.logits)[at(u)];
-  } else if (tc.dtype == 1) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) e.t[u] = to_f(static_cast<const bf16_t*>(tc.logits)[at(u)]);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) e.t[u] = to_f(static_cast<const f16_t*>(tc.logits)[at(u)]);
-  }
-#pragma unroll
-  for (int u = 0; u < 8; ++u) e.has[u] = j0 + u < tc.k && e.id[u] >= 0 && !(e.t[u] == NEG_INF);
-  return e;
-}
+// if asked for.
 template <typename T, int M>
 __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows, int V, Teacher tc, Ids targets,
                                                       int64_t ignore, Mix mix, Upstream up,
