@@ -628,7 +628,7 @@ int ghm_zsc_logits(const float* i_emb, int64_t n_rows, const float* t_emb, int D
  * point atomics).  ws: scratch of at least the matching *_ws bytes (16-byte aligned,
  * NULL where that is 0), not shared by calls that may run at the same time.
  *
- * A row whose target is ignore_index is padding: its logits are never read, its
+ * A row whose target is ignore_index is padding: its logits are not used, its
  * results and gradient are 0 (top_id -1).  A target outside 0 .. V - 1 makes its own
  * row NaN.  A logit of -inf has probability 0; a row whose maximum is not finite has no
  * distribution and is NaN, as log_softmax has it. */

@@ -1,6 +1,7 @@
 """The token operators (csrc/ghm_score.hip, ghm_distill.hip, ghm_embed.hip) against their definitions in 64 bits
 (oracle/token_oracle.py, which also gives the bound that a 32-bit evaluation with one
 final rounding may be off; the values below are never measured ones)."""
+import gc
 import math
 
 import pytest
@@ -20,6 +21,13 @@ def _need_gpu():
         pytest.skip("no HIP device")
     from ghmclip import _native
     assert _native.hip_lib().ghm_device_ok() == 1
+    torch.cuda.synchronize()  # what ran before this file has ended
+    gc.collect()
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.synchronize()
+    gc.collect()
+    torch.cuda.empty_cache()  # up to 40 GB
 
 
 def _M():
