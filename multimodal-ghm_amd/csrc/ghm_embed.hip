@@ -34,8 +34,7 @@ __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&x
 }
 
 // A block takes `per` rows of `vecs` vectors; lanes take vectors in turn.  Bound by the
-// writes: 16,384 tokens x 2048 bf16 in 17 us (67 MB each way, the read one mostly cached),
-// 131,071 x 1001 f32 in 127 us (525 MB written at 4.1 TB/s).
+// writes: 16,384 tokens x 2048 bf16 in 17 us (67 MB each way, the read one mostly cached).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict__ weight, int64_t w_stride,
                                                     float scale, T* __restrict__ out, int64_t N, int64_t V, int D,
@@ -62,6 +61,84 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
       for (int i = 0; i < VE; ++i) x[u][i] *= f;
       store_cols<T, VE, STREAM>(out + (i0 + t / vecs) * D, edge_col<VE>(t % vecs * VE, D), D, x[u]);
     }
+  }
+}
+
+// The same for large outputs whose rows are not whole lines (D >= VE): the output is one run of
+// N * D values in vectors of VE from its first 16-byte boundary on, 256 * U of them per
+// block, so that lines are written whole and past the caches, whatever D is.  A vector that crosses
+// from a row into the next is put together from the one's last VE values and the other's
+// first.  131,071 x 1001 f32 in 102 us (5.1 TB/s; 129 row by row), 131,071 x 2047 bf16
+// in 114 (151); what fits the 256 MB cache is sooner there by rows: 10,000 x 1001 f32 in 11 us
+// (21), 100,000 x 1001 bf16 in 41 (51).
+constexpr int64_t RUN_BYTES = int64_t(1) << 28;
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_run(Ids tok, const T* __restrict__ weight, int64_t w_stride, float scale,
+                                                   T* __restrict__ out, int64_t N, int64_t V, uint32_t D, int head,
+                                                   int64_t vecs) {
+  constexpr int VE = Vec<T>::N, U = 4;
+  using raw = typename Vec<T>::raw;
+  const auto start = [&](int64_t t) { return weight + (t >= 0 && t < V ? t : 0) * w_stride; };  // a bad token reads row 0
+  const auto factor = [&](int64_t t) { return t >= 0 && t < V ? scale : __builtin_nanf(""); };
+  if (blockIdx.x == 0) {  // the values before the first vector and after the last one
+    const int t = threadIdx.x;
+    const int64_t e = t < head ? t : head + vecs * VE + t - head;
+    if (t < head + VE && e < N * D) {
+      const int64_t v = ld_id(tok, e / D);
+      from_f(out[e], to_f(start(v)[e % D]) * factor(v));
+    }
+  }
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x) * (256 * U), e0 = head + j0 * VE, r0 = e0 / D;
+  const uint32_t c0 = static_cast<uint32_t>(e0 - r0 * D);
+  int64_t v[U], next[U];
+  uint32_t col[U], row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {  // past the end: the last vector again
+    const int64_t j = j0 + threadIdx.x + 256 * u;
+    const uint32_t o = c0 + static_cast<uint32_t>((j < vecs ? j : vecs - 1) - j0) * VE;
+    row[u] = o / D;
+    col[u] = o - row[u] * D;
+  }
+  ld_ids<U>(tok, v, [&](int u) { return r0 + row[u]; });
+  ld_ids<U>(tok, next, [&](int u) { return r0 + row[u] + 1 < N ? r0 + row[u] + 1 : N - 1; });
+  u32x4 x[U], y[U];
+  bool in[U];
+  const auto scaled = [&](u32x4 p, float f) {
+    float z[VE];
+    T e[VE];
+    unpack<T>(p, z);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) from_f(e[i], z[i] * f);
+    __builtin_memcpy(&p, e, 16);
+    return p;
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    in[u] = col[u] + VE <= D;
+    x[u] = *reinterpret_cast<const raw*>(start(v[u]) + (in[u] ? col[u] : D - VE));
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) y[u] = in[u] ? x[u] : *reinterpret_cast<const raw*>(start(next[u]));
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t j = j0 + threadIdx.x + 256 * u;
+    if (j >= vecs) break;
+    u32x4 o = scaled(x[u], factor(v[u]));
+    if (!in[u]) {
+      const u32x4 q = scaled(y[u], factor(next[u]));
+      const uint32_t k = col[u] - (D - VE), words = k * sizeof(T) / 4;  // k values of x[u] are before this vector
+      uint32_t z[8] = {o[0], o[1], o[2], o[3], q[0], q[1], q[2], q[3]};
+#pragma unroll
+      for (int i = 0; i < 6; ++i) z[i] = words & 2 ? z[i + 2] : z[i];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) z[i] = words & 1 ? z[i + 1] : z[i];
+      if (sizeof(T) == 2 && (k & 1)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = z[i] >> 16 | z[i + 1] << 16;
+      }
+      o = u32x4{z[0], z[1], z[2], z[3]};
+    }
+    __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(out + head + j * VE));
   }
 }
 
@@ -613,7 +690,14 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
   const Ids t{tokens, id_bits};
   const int d = static_cast<int>(D);
   hipStream_t s = ghm_stream(stream);
-  if (whole_lines(out, D * (16 / ve)))
+  const int64_t size = 16 / ve;
+  if (!whole_lines(out, D * size) && D >= ve && N * D * size > RUN_BYTES) {
+    const int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(out) % 16) % 16 / size);
+    const int64_t run = (N * D - head) / ve;
+    TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_run<T>, dim3(static_cast<unsigned>((run + 1023) / 1024)), b, 0, s, t,
+                                           static_cast<const T*>(weight), w_stride, scale, static_cast<T*>(out), N, V,
+                                           static_cast<uint32_t>(D), head, run));
+  } else if (whole_lines(out, D * size))
     TOK_DISPATCH(dtype, hipLaunchKernelGGL((k_embed_rows<T, true>), g, b, 0, s, t, static_cast<const T*>(weight), w_stride,
                                            scale, static_cast<T*>(out), N, V, d, vecs, per));
   else

@@ -629,6 +629,38 @@ def test_embedding_of_padding_alone(N, V):
     assert (dw == 0).all()
 
 
+@pytest.mark.parametrize("dtype,N,D", [(torch.float32, 67201, 1001), (torch.bfloat16, 131071, 1030),
+                                       (torch.float16, 140001, 961), (torch.bfloat16, 9600001, 15),
+                                       (torch.float32, 13500001, 5)])
+def test_embedding_of_large_outputs(dtype, N, D):
+    """Outputs of more than 256 MB with rows that are not whole lines, from an aligned address
+    and from others: one rounded product per value, and nothing beside the output is written."""
+    M = _M()
+    from ghmclip.models import token_ops as T
+    V = 301
+    g = torch.Generator().manual_seed(D)
+    w = torch.randn(V, D, generator=g).to(dtype).to(DEV)
+    tok = torch.randint(0, V, (N,), generator=g)
+    bad = torch.tensor([0, 7, 8, N // 2, N - 1])
+    tok[bad] = torch.tensor([V, -1, V + 5, -7, 1 << 40])
+    tok = tok.to(DEV)
+    ok = (tok >= 0) & (tok < V)
+    rows = (w.float() * 1.5).to(dtype)
+
+    def check(out):
+        for a in range(0, N, 1 << 20):
+            o, t, k = out[a:a + (1 << 20)], tok[a:a + (1 << 20)], ok[a:a + (1 << 20)]
+            assert torch.equal(o[k], rows[t[k]])
+            assert o[~k].isnan().all()
+    check(M.scaled_embedding(tok, w, 1.5))
+    for off in (1, 3):
+        buf = torch.full((N * D + 64,), 7., dtype=dtype, device=DEV)
+        T._call(buf.device, "ghm_embed_rows_fwd", tok.data_ptr(), 64, w.data_ptr(), T._DTYPE[dtype], D, 1.5,
+                buf.data_ptr() + off * buf.element_size(), N, V, D)
+        check(buf[off:off + N * D].view(N, D))
+        assert (buf[:off] == 7).all() and (buf[off + N * D:] == 7).all()
+
+
 def test_embedding_gradient_of_two_strides():
     M = _M()
     g = torch.Generator().manual_seed(2)
