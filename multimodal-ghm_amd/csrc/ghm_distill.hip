@@ -273,8 +273,8 @@ __device__ __forceinline__ void distill_row_grad(const T* z, T* d, int lo, int h
     zero_row<T, N, W>(d, lo, hi, w, lane);
     return;
   }
-  if (g.two) map_row<T, N, U, W, true>(z, d, lo, hi, w, lane, [=](float x) { return g.both(x); });
-  else map_row<T, N, U, W, true>(z, d, lo, hi, w, lane, [=](float x) { return g.one(x); });
+  if (g.two) map_row<T, N, U, W, true, false>(z, d, lo, hi, w, lane, [=](float x) { return g.both(x); });
+  else map_row<T, N, U, W, true, false>(z, d, lo, hi, w, lane, [=](float x) { return g.one(x); });
   group_sync<W>();
   distill_entries<T, W>(z, d, lo, hi, tc, mix, g, lds, y, w, lane);
 }
@@ -477,7 +477,8 @@ __global__ __launch_bounds__(256) void k_distill_join(Rows rows, int V, Teacher 
     row_stats[r] = make_float4(a.m, l1, l2, 1.f);
   }
 }
-// ... and the gradient from the row's statistics
+// ... and the gradient from the row's statistics, the last rows first (what the sums read last is
+// still in the 256 MB cache: loss and gradient of 2,048 rows of 65,536 f32 values 297 us, 316 in order)
 template <typename T, int N, int U, int W>
 __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows, int V, Teacher tc, Ids targets,
                                                       int64_t ignore, Mix mix, Upstream up, int parts, int part_len,
@@ -485,8 +486,9 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
   constexpr int G = 4 / W;
   __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W, r = item / parts;
-  if (r >= n_rows) return;
+  const int64_t item = n_rows * parts - 1 - (static_cast<int64_t>(blockIdx.x) * G + wave / W);
+  if (item < 0) return;
+  const int64_t r = item / parts;
   const int lo = static_cast<int>(item % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
   T* d = dz + r * V;
   const float4 st = row_stats[r];
