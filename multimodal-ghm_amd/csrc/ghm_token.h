@@ -179,8 +179,9 @@ __device__ __forceinline__ float group_sum(float v, float* slot, int w) {
 //   s = sum e^{c1 (z - m)};  SECOND_ENT: t = sum e^{c1 d} d (d = z - m);
 //   SECOND_EXP: t = sum e^{c2 d};  SECOND_NONE: t unused.
 // The maximum starts at the lowest finite value, so differences never are -inf minus
-// -inf; a difference is cut at -1e4 where it is a factor (e^-1e4 = 0).  NaN and +inf
-// make s NaN.  c1, c2 carry log2 e.
+// -inf; where a difference is a factor of the entropy's sum it is cut at -1e4 (e^-1e4 = 0, and
+// 0 times -inf is not).  An exponent's difference is never cut: c1 and c2 carry log2 e over a
+// temperature of up to 10^6, where e^(-1e4 / 10^6) is 0.99.  NaN and +inf make s NaN.
 // EXACT: values at the maximum are counted in n and not added to the sums, so that the
 // logarithm of a sum just above 1 keeps its digits (log1p): a row with one likely value
 // of few.  Rows of up to 256 values afford the two instructions per value.
@@ -193,9 +194,9 @@ struct Sums {
 };
 template <int SECOND>
 __device__ __forceinline__ void rebase(Sums& a, float m, float c1, float c2) {
-  const float dm = fmaxf(a.m - m, -1e4f), f = __builtin_amdgcn_exp2f(dm * c1);
+  const float dm = a.m - m, f = __builtin_amdgcn_exp2f(dm * c1);
   const float n = dm == 0.f ? 0.f : a.n;  // what was at the old maximum joins the sums
-  if constexpr (SECOND == SECOND_ENT) a.t = f * (a.t + dm * (a.s + n));
+  if constexpr (SECOND == SECOND_ENT) a.t = f * (a.t + fmaxf(dm, -1e4f) * (a.s + n));
   if constexpr (SECOND == SECOND_EXP) a.t = __builtin_amdgcn_exp2f(dm * c2) * (a.t + n);
   a.s = f * (a.s + n);
   a.n -= n;

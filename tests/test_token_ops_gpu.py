@@ -416,6 +416,58 @@ def test_distill_special_values(V):
         assert torch.isnan(dz[2:6]).any(-1).all() and torch.isfinite(dz[[0, 1, 6, 7]]).all() and (dz[7] == 0).all()
 
 
+def _spread_rows(V, dtype, seed):
+    """Rows whose values lie far apart, (logits, ids, teacher's logits, targets): finite masks that end or
+    begin inside a lane's, a wave's or a part's values, and values of tens of thousands.  The teacher's
+    entries and the targets are values that no mask holds."""
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(7, V, generator=g) * 3
+    z[4] = (torch.randn(V, generator=g) * 2e4).clamp(-6e4, 6e4)
+    z[5] = torch.linspace(-6e4, 6e4, V)          # the maximum rises with every step
+    low = torch.finfo(dtype).min
+    masks = torch.zeros(7, V, dtype=torch.bool)
+    masks[0, :V // 2] = True
+    masks[1, V // 2:] = True
+    masks[2, ::2] = True
+    masks[3, :V - 1] = True                      # one value left, the last
+    z = z.to(dtype)
+    z[masks] = low
+    z[2, 1::4] = -1e4 * (2 if dtype == torch.float16 else 1e3)
+    k = min(V // 2, 5)
+    ids = torch.stack([(~m).nonzero()[:, 0][torch.randint(0, int((~m).sum()), (k,), generator=g)] for m in masks])
+    ids[2] = ids[2] // 4 * 4 + 3 if V >= 8 else ids[2]
+    ids[2].clamp_(max=(V - 4) // 4 * 4 + 3)
+    return z, ids, torch.randn(7, k, generator=g) * 2, ids[:, 0].clone()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tau", [1e-6, 1e-3, 20.0, 1e3, 1e4, 1e6])
+@pytest.mark.parametrize("V", [10, 100, 700, 3000, 9001, 40000, 70001, 140001, 300001])
+def test_distill_temperatures_with_values_far_apart(V, tau, dtype):
+    """Both ends of the accepted temperatures: what is e^-10000 at a temperature of 1 is 0.99 at one
+    of 10^6, in rows of one lane, one wave, several waves and parts; the loss alone, the loss with its gradient
+    and the gradient from saved statistics, each against the definition."""
+    M = _M()
+    z, ids, t, y = _spread_rows(V, dtype, V)
+    # a gradient is alpha temperature (p - q): times a power of two that keeps it within f16
+    up = 2.0 ** -20 if tau == 1e6 else 1.0
+    for alpha in (1.0, 0.5):
+        yy = y if alpha < 1 else None
+        r = O.distill(z.double(), ids, t.double(), yy, tau, alpha)
+        on = [z.to(DEV), ids.to(DEV), t.to(DEV), None if yy is None else yy.to(DEV)]
+        opts = dict(temperature=tau, alpha=alpha, reduction="none")
+        want, bound = up * r["dz"], up * (r["bdz"] + 4 * O.U * r["dz"].abs())
+        loss, dz = M.distill_loss_and_grad(*on, grad_scale=up, **opts)
+        _near(loss, r["row_loss"], r["brow_loss"], f"alpha {alpha}, step")
+        _grad_near(dz, want, bound, dtype, f"alpha {alpha}, step's gradient")
+        _near(M.distill_loss(*on, **opts), r["row_loss"], r["brow_loss"], f"alpha {alpha}, loss alone")
+        leaf = on[0].requires_grad_()
+        loss = M.distill_loss(leaf, *on[1:], **opts)
+        _near(loss, r["row_loss"], r["brow_loss"], f"alpha {alpha}, loss")
+        dz, = torch.autograd.grad(loss, leaf, torch.full_like(loss, up))
+        _grad_near(dz, want, bound, dtype, f"alpha {alpha}, autograd")
+
+
 def test_distill_nothing_counts():
     M = _M()
     z = _logits(5, 77, torch.float32, 0).to(DEV).requires_grad_()
