@@ -7,12 +7,14 @@ have no counterpart in the reference.  Logits, tables and gradients are float32,
 bfloat16 or float16 on a HIP device; sums, statistics and losses are float32.  Work
 is issued on the current stream of the tensors' device; nothing synchronises, so
 token ids are not checked on the host: an id outside the vocabulary gives NaN in
-its own row (and adds nothing to an embedding gradient).
+its own row (and adds nothing to an embedding gradient).  Gradients are of first order and
+reverse mode; a second one and forward-mode tangents raise.
 """
 from collections import namedtuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from .. import _native
 from .hip_encoder import require_hip
@@ -92,7 +94,18 @@ def _call(device, name, *args):
     return _native.call(name, *args, _raw_stream(device.index))
 
 
+def _check_tangent(t, what):
+    """Forward-mode tangents are refused: a dual tensor without requires_grad takes the calls past
+    autograd, whose results would carry none (derivative 0).  Asked only while a level of
+    forward-mode differentiation is open (0.1 us a call in place of 0.9)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not offered")
+
+
 def _check_logits(logits):
+    _check_tangent(logits, "logits")
     require_hip(logits)
     code = _dtype(logits, "logits")
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -350,6 +363,7 @@ def scaled_embedding(tokens, weight, scale=1.0, padding_idx=None):
     each token in float32, in the order they appear (sorted tokens, no atomics: the same
     bits every run), and rounds once; row ``padding_idx`` gets none.  A token outside
     0 .. V - 1 gives a NaN row and adds nothing to the gradient."""
+    _check_tangent(weight, "weight")
     require_hip(weight)
     _dtype(weight, "weight")
     if weight.dim() != 2 or 0 in weight.shape:

@@ -119,6 +119,22 @@ def test_wrappers_refuse_cpu_tensors():
         M.TopLogitsDistillLoss(reduction="median")
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor needs no gradient, and a result without a tangent reads as derivative 0."""
+    import torch.autograd.forward_ad as fwAD
+    from ghmclip import models as M
+    z, ids, t = torch.zeros(2, 5), torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 1)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(z, torch.ones_like(z))
+        for f in (lambda: M.token_logprobs(dual), lambda: M.distill_loss(dual, ids, t),
+                  lambda: M.distill_loss_and_grad(dual, ids, t), lambda: M.TopLogitsDistillLoss()(dual, ids, t),
+                  lambda: M.scaled_embedding(ids, dual)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+
+
 def test_limits_match_the_header():
     import os
     import re
