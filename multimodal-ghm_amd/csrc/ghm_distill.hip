@@ -220,6 +220,12 @@ __device__ __forceinline__ float distill_row_loss(const T* z, int V, const Teach
   return loss;
 }
 
+// the factor of the teacher's part of the gradient: none without entries, but a row that is NaN stays so
+__device__ __forceinline__ float teacher_scale(const Mix& mix, bool some, float scale) {
+  if (scale != scale) return scale;
+  return some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : 0.f;
+}
+
 // The gradient of a row: the two softmaxes everywhere, then the teacher's and the target's
 // entries again.
 struct DistillGrad {
@@ -234,7 +240,7 @@ struct DistillGrad {
 };
 __device__ __forceinline__ DistillGrad distill_grad(const Mix& mix, bool some, float m, float l1, float l2, float scale) {
   DistillGrad g;
-  g.A = some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : 0.f;
+  g.A = teacher_scale(mix, some, scale);
   g.B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
   g.AB = g.A + g.B;
   g.m = m;
@@ -586,7 +592,7 @@ __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows,
   }
   if (!dz) return;
   if (bad) scale = __builtin_nanf("");
-  const float A = some && mix.alpha != 0.f ? scale * mix.alpha * mix.tau : bad ? scale : 0.f;
+  const float A = teacher_scale(mix, some, scale);
   const float B = mix.hard ? scale * (1.f - mix.alpha) : 0.f;
 #pragma unroll
   for (int v = 0; v < M; ++v) {

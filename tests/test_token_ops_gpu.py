@@ -468,6 +468,19 @@ def test_distill_temperatures_with_values_far_apart(V, tau, dtype):
         _grad_near(dz, want, bound, dtype, f"alpha {alpha}, autograd")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [10, 33, 100, 300, 3000, 9000, 40000, 140001])
+def test_distill_bad_targets_without_entries(V, dtype):
+    """alpha = 1 and no teacher's entry: a target outside the vocabulary makes its row NaN, the gradient's
+    too, in rows of every length; one that holds only that it counts is 0."""
+    z, y = _logits(6, V, dtype, V), torch.tensor([1, V, -1, V - 1, -100, 1 << 40])
+    ids, t = _teacher(6, V, 4, V, ragged=False)
+    ids[[1, 3, 4]] = -1
+    t[2] = -math.inf
+    for tau in (1.0, 2.0):
+        _check_distill(z, ids, t, y, tau, 1.0, dtype, f"tau {tau}")
+
+
 def test_distill_nothing_counts():
     M = _M()
     z = _logits(5, 77, torch.float32, 0).to(DEV).requires_grad_()
