@@ -220,6 +220,11 @@ __device__ __forceinline__ float distill_row_loss(const T* z, int V, const Teach
   return loss;
 }
 
+// A row that is NaN, loss and gradient: an entry or the target lies outside the vocabulary, or the row
+// has no distribution (no finite maximum: the logarithm of its sum, l2, is not finite).
+__device__ __forceinline__ bool row_bad(bool bad_entry, const Ids& targets, int64_t y, int V, float l2) {
+  return bad_entry || (targets.p && (y < 0 || y >= V)) || !(l2 - l2 == 0.f);
+}
 // the factor of the teacher's part of the gradient: none without entries, but a row that is NaN stays so
 __device__ __forceinline__ float teacher_scale(const Mix& mix, bool some, float scale) {
   if (scale != scale) return scale;
@@ -323,7 +328,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
   a = group_join<SECOND, W>(a, slots, w, mix.c1, mix.c2);
   const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
-  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  const bool bad = row_bad(tr.bad, targets, y, V, l2);
   if (w == 0 && lane == 0) {
     row_loss[r] = bad ? __builtin_nanf("") : loss;
     row_stats[r] = make_float4(a.m, l1, l2, 1.f);
@@ -407,7 +412,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
   if constexpr (TWO) a.t = group_sum<W>(a.t, slots + 2 * W, w);
   const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   const float loss = distill_row_loss<T, W>(z, V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
-  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  const bool bad = row_bad(tr.bad, targets, y, V, l2);
   if (w == 0 && lane == 0) {
     row_loss[r] = bad ? __builtin_nanf("") : loss;
     row_stats[r] = make_float4(a.m, l1, l2, 1.f);
@@ -479,7 +484,7 @@ __global__ __launch_bounds__(256) void k_distill_join(Rows rows, int V, Teacher 
   const float l1 = a.log_s(), l2 = TWO ? a.log_t() : l1;
   const float loss = distill_row_loss<T, 4>(row_ptr<T>(rows, r), V, tc, r, mix, tr, lds, a.m, l1, l2, y, w, lane);
   if (threadIdx.x == 0) {
-    row_loss[r] = tr.bad || (targets.p && (y < 0 || y >= V)) ? __builtin_nanf("") : loss;
+    row_loss[r] = row_bad(tr.bad, targets, y, V, l2) ? __builtin_nanf("") : loss;
     row_stats[r] = make_float4(a.m, l1, l2, 1.f);
   }
 }
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
   const int64_t y = targets.p ? ld_id(targets, r) : -1;
   const TeacherLds<W> lds = teacher_at<W>(wave / W, tc.k, teach_slots[wave / W]);
   const TeacherRow tr = teacher_row<W>(tc, r, V, mix.it, lds, w, lane);
-  const bool bad = tr.bad || (targets.p && (y < 0 || y >= V));
+  const bool bad = row_bad(tr.bad, targets, y, V, st.z);
   distill_row_grad<T, N, U, W>(
       row_ptr<T>(rows, r), d, lo, hi, tc, mix,
       distill_grad(mix, tr.some, st.x, st.y, st.z, bad ? __builtin_nanf("") : upstream(up, r, lane)), lds, y, w, lane);
@@ -531,7 +536,7 @@ __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows,
     for (int v = 0; v < M; ++v) x[v] = v < V ? to_f(z[v]) : NEG_INF;
   }
   float mt = -FLT_MAX;
-  bool some = false, bad = targets.p && (y < 0 || y >= V);
+  bool some = false, bad = false;
   for (int j0 = 0; j0 < tc.k; j0 += 8) {
     const Entries e = ld_entries(tc, first, j0);
 #pragma unroll
@@ -559,6 +564,7 @@ __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows,
   }
   fold<SECOND_EXP, true>(a, x, LOG2E, mix.c2);
   const float l1 = a.log_s(), l2 = a.log_t();
+  bad = row_bad(bad, targets, y, V, l2);
   float st = 0.f, kl = 0.f;
   for (int j0 = 0; j0 < tc.k; j0 += 8) {
     const Entries e = ld_entries(tc, first, j0);

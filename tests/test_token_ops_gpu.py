@@ -481,6 +481,28 @@ def test_distill_bad_targets_without_entries(V, dtype):
         _check_distill(z, ids, t, y, tau, 1.0, dtype, f"tau {tau}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [10, 33, 100, 300, 3000, 9000, 40000, 140001])
+def test_distill_rows_without_a_distribution(V, dtype):
+    """A row without a finite maximum is NaN, loss and gradient, whether or not the teacher has an
+    entry there and whatever the gradient is scaled with."""
+    M = _M()
+    z, y = _logits(8, V, dtype, V), torch.zeros(8, dtype=torch.long)
+    ids, t = _teacher(8, V, 4, V, ragged=False)
+    z[:3] = -math.inf
+    z[3, V - 1] = math.nan
+    z[4, V // 2] = math.inf
+    ids[[0, 3, 4, 5]] = -1
+    y[2] = -100
+    for tau, alpha in ((1.0, 1.0), (2.0, 1.0), (1.0, 0.5), (2.0, 0.5), (2.0, 0.0)):
+        _check_distill(z, ids, t, y, tau, alpha, dtype, f"tau {tau} alpha {alpha}")
+        loss, dz = M.distill_loss_and_grad(z.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV), temperature=tau, alpha=alpha,
+                                           reduction="none", grad_scale=0.0)
+        bad = torch.tensor([True, True, False, True, True, False, False, False])
+        assert torch.equal(loss.isnan().cpu(), bad) and torch.equal(dz.isnan().all(-1).cpu(), bad)
+        assert (dz[~bad] == 0).all()
+
+
 def test_distill_nothing_counts():
     M = _M()
     z = _logits(5, 77, torch.float32, 0).to(DEV).requires_grad_()
