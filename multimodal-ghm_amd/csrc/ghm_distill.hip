@@ -618,7 +618,7 @@ __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows,
   GHM_CHECK(!targets || ids_ok(target_bits), "target_bits (8, 32, 64)");                                        \
   GHM_CHECK(k >= 1 && k <= GHM_DISTILL_MAX, "k (1 .. 1024)");                                                   \
   GHM_CHECK(temperature >= 1e-6f && temperature <= 1e6f, "temperature (1e-6 .. 1e6)");                 \
-  GHM_CHECK(alpha >= 0.f && alpha <= 1.f && (targets || alpha == 1.f), "alpha (0 .. 1; below 1 needs targets)")
+  GHM_CHECK(alpha >= 0.f && alpha <= 1.f && (targets || alpha == 1.f || rows == 0), "alpha (0 .. 1; below 1 needs targets)")
 
 namespace {
 struct Distill {

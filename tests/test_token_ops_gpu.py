@@ -518,6 +518,22 @@ def test_distill_nothing_counts():
     assert M.distill_loss(z.detach()[:0], ids[:0], t[:0], reduction="none").shape == (0,)
 
 
+@pytest.mark.parametrize("V", [10, 77, 3000])
+def test_distill_empty_batch_with_hard_labels(V):
+    """No row at all, with targets and alpha below 1: the loss of nothing and an empty gradient."""
+    M = _M()
+    z = torch.zeros(0, V, device=DEV, requires_grad=True)
+    ids, t = torch.zeros(0, 3, dtype=torch.long, device=DEV), torch.zeros(0, 3, device=DEV)
+    y = torch.zeros(0, dtype=torch.long, device=DEV)
+    for reduction in ("mean", "sum", "none"):
+        loss = M.distill_loss(z, ids, t, y, alpha=0.5, temperature=2.0, reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ()) and (loss == 0).all()
+        dz, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+        assert dz.shape == z.shape
+        loss, dz = M.distill_loss_and_grad(z.detach(), ids, t, y, alpha=0.5, reduction=reduction)
+        assert (loss == 0).all() and dz.shape == z.shape
+
+
 def test_distill_views_and_module():
     M = _M()
     base = _logits(24, 37, torch.bfloat16, 3).view(4, 6, 37)

@@ -81,6 +81,13 @@ def test_distill_bwd_refusals(kw):
     assert _distill_bwd(**kw) == -22
 
 
+def test_distill_of_no_rows_takes_null_targets():
+    """An empty batch's buffers are null, its targets among them."""
+    none = dict(rows=0, logits=None, ids=None, t=None, y=None, dz=None, alpha=0.5)
+    assert _distill(**none, row_loss=None, reduction=0) != -22  # (no device here to ask for a launch error)
+    assert _distill_bwd(**none, g=None) == 0
+
+
 def _embed(**kw):
     a = dict(tok=P, bits=64, w=P, dtype=0, ws=8, scale=1.0, out=P, N=4, V=10, D=8, stream=None)
     a.update(kw)
