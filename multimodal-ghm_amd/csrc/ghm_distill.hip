@@ -307,7 +307,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(Rows rows, in
   __shared__ float slots[3 * W];
   __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  const int64_t r = block_number() * G + wave / W;
   if (r >= n_rows) return;
   T* d = dz ? dz + r * V : nullptr;
   if (!row_counts(tc, targets, ignore, r, lane)) {
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, R == 16 ? 4 : 1) void k_dist
   __shared__ float slots[3 * W];
   __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  const int64_t r = block_number() * G + wave / W;
   if (r >= n_rows) return;
   T* d = dz + r * V;
   if (!row_counts(tc, targets, ignore, r, lane)) {
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(256) void k_distill_grad(Rows rows, int64_t n_rows,
   constexpr int G = 4 / W;
   __shared__ float teach_slots[G][4 * W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t item = n_rows * parts - 1 - (static_cast<int64_t>(blockIdx.x) * G + wave / W);
+  const int64_t item = n_rows * parts - 1 - (block_number() * G + wave / W);
   if (item < 0) return;
   const int64_t r = item / parts;
   const int lo = static_cast<int>(item % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
@@ -651,7 +651,7 @@ inline Mix make_mix(bool targets, float tau, float alpha) {
 template <typename T, int N, int U, int W>
 void launch_distill(const Distill& a, const Upstream& up, T* dz) {
   constexpr int G = W == 1 ? 4 : 1;
-  const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
+  const dim3 g = grid_of((a.rows + G - 1) / G, 64 * G * W), b(64 * G * W);
   if (a.mix.two)
     hipLaunchKernelGGL((k_distill<T, N, U, W, true>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
@@ -662,7 +662,7 @@ void launch_distill(const Distill& a, const Upstream& up, T* dz) {
 template <typename T, int R, int W>
 void launch_step(const Distill& a, const Upstream& up, T* dz) {
   constexpr int G = W == 1 ? 4 : 1;
-  const dim3 g(static_cast<unsigned>((a.rows + G - 1) / G)), b(64 * G * W);
+  const dim3 g = grid_of((a.rows + G - 1) / G, 64 * G * W), b(64 * G * W);
   if (a.mix.two)
     hipLaunchKernelGGL((k_distill_step<T, R, W, true>), g, b, 8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up,
                        a.row_loss, a.stats, dz);
@@ -673,8 +673,8 @@ void launch_step(const Distill& a, const Upstream& up, T* dz) {
 template <typename T, int N, int U, int W>
 void launch_distill_grad(const Distill& a, const Upstream& up, const Split& p, T* dz) {
   constexpr int G = 4 / W;
-  hipLaunchKernelGGL((k_distill_grad<T, N, U, W>), dim3(static_cast<unsigned>((a.rows * p.parts + G - 1) / G)), dim3(256),
-                     8 * a.tc.k * G, a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up, p.parts, p.len, a.stats, dz);
+  hipLaunchKernelGGL((k_distill_grad<T, N, U, W>), grid_of((a.rows * p.parts + G - 1) / G, 256), dim3(256), 8 * a.tc.k * G,
+                     a.s, a.m, a.rows, a.V, a.tc, a.t, a.ignore, a.mix, up, p.parts, p.len, a.stats, dz);
 }
 template <typename T>
 void distill_short(const Distill& a, const Upstream& up, float* row_loss, T* dz) {

@@ -40,7 +40,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
                                                     float scale, T* __restrict__ out, int64_t N, int64_t V, int D,
                                                     int vecs, int per) {
   constexpr int VE = Vec<T>::N, U = 4;
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per;
+  const int64_t i0 = block_number() * per;
+  if (i0 >= N) return;
   const int n = static_cast<int>(N - i0 < per ? N - i0 : per) * vecs;
   for (int t0 = threadIdx.x; t0 < n; t0 += 256 * U) {
     int64_t v[U];
@@ -80,7 +81,9 @@ __global__ __launch_bounds__(256) void k_embed_run(Ids tok, const T* __restrict_
   using raw = typename Vec<T>::raw;
   const auto start = [&](int64_t t) { return weight + (t >= 0 && t < V ? t : 0) * w_stride; };  // a bad token reads row 0
   const auto factor = [&](int64_t t) { return t >= 0 && t < V ? scale : __builtin_nanf(""); };
-  if (blockIdx.x == 0) {  // the values before the first vector and after the last one
+  const int64_t j0 = block_number() * (256 * U), e0 = head + j0 * VE, r0 = e0 / D;
+  if (j0 >= vecs) return;
+  if (j0 == 0) {  // the values before the first vector and after the last one
     const int t = threadIdx.x;
     const int64_t e = t < head ? t : head + vecs * VE + t - head;
     if (t < head + VE && e < N * D) {
@@ -88,7 +91,6 @@ __global__ __launch_bounds__(256) void k_embed_run(Ids tok, const T* __restrict_
       from_f(out[e], to_f(start(v)[e % D]) * factor(v));
     }
   }
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x) * (256 * U), e0 = head + j0 * VE, r0 = e0 / D;
   const uint32_t c0 = static_cast<uint32_t>(e0 - r0 * D);
   int64_t v[U], next[U];
   uint32_t col[U], row[U];
@@ -686,7 +688,7 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
   if (N == 0) return GHM_OK;
   const int ve = dtype == 0 ? 4 : 8, vecs = static_cast<int>((D + ve - 1) / ve);
   const int per = vecs >= 1024 ? 1 : 1024 / vecs;
-  const dim3 g(static_cast<unsigned>((N + per - 1) / per)), b(256);
+  const dim3 g = grid_of((N + per - 1) / per, 256), b(256);
   const Ids t{tokens, id_bits};
   const int d = static_cast<int>(D);
   hipStream_t s = ghm_stream(stream);
@@ -694,7 +696,7 @@ extern "C" int ghm_embed_rows_fwd(const void* tokens, int id_bits, const void* w
   if (!whole_lines(out, D * size) && D >= ve && N * D * size > RUN_BYTES) {
     const int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(out) % 16) % 16 / size);
     const int64_t run = (N * D - head) / ve;
-    TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_run<T>, dim3(static_cast<unsigned>((run + 1023) / 1024)), b, 0, s, t,
+    TOK_DISPATCH(dtype, hipLaunchKernelGGL(k_embed_run<T>, grid_of((run + 1023) / 1024, 256), b, 0, s, t,
                                            static_cast<const T*>(weight), w_stride, scale, static_cast<T*>(out), N, V,
                                            static_cast<uint32_t>(D), head, run));
   } else if (whole_lines(out, D * size))

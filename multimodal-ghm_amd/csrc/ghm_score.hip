@@ -158,7 +158,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 4) void k_score(Rows rows, i
   __shared__ float slots[W == 1 ? 1 : 3 * W];
   __shared__ TopLds<N, TOP ? W : 1> top_lds[TOP ? G : 1];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * G + wave / W;
+  const int64_t item = block_number() * G + wave / W;
   const int64_t r = part_sums ? item / parts : item;
   if (r >= n_rows) return;
   const int64_t y = targets.p ? ld_id(targets, r) : 0;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256) void k_score_bwd(Rows rows, int64_t n_rows, in
                                                    ScoreGrad g, int parts, int part_len, T* __restrict__ dz) {
   constexpr int G = 4 / W;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % W;
-  const int64_t item = n_rows * parts - 1 - (static_cast<int64_t>(blockIdx.x) * G + wave / W);
+  const int64_t item = n_rows * parts - 1 - (block_number() * G + wave / W);
   if (item < 0) return;
   const int64_t r = item / parts;
   const int lo = static_cast<int>(item % parts) * part_len, hi = lo + part_len < V ? lo + part_len : V;
@@ -392,7 +392,7 @@ void launch_score(const Rows& m, int64_t rows, int V, const Ids& t, int64_t igno
   constexpr int G = W == 1 ? 4 : 1;
   float4* sums = p.parts > 1 ? static_cast<float4*>(ws) : nullptr;
   uint64_t* keys = sums ? reinterpret_cast<uint64_t*>(sums + rows * p.parts) : nullptr;
-  const dim3 g(static_cast<unsigned>((rows * p.parts + G - 1) / G)), b(64 * G * W);
+  const dim3 g = grid_of((rows * p.parts + G - 1) / G, 64 * G * W), b(64 * G * W);
   if (o.top_k)
     hipLaunchKernelGGL((k_score<T, N, U, W, true>), g, b, 0, s, m, rows, V, t, ignore, o, p.parts, p.len, sums, keys);
   else
@@ -453,8 +453,8 @@ template <typename T, int N, int U, int W>
 void launch_score_bwd(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreGrad& g,
                       const Split& p, T* dz, hipStream_t s) {
   constexpr int G = 4 / W;
-  hipLaunchKernelGGL((k_score_bwd<T, N, U, W>), dim3(static_cast<unsigned>((rows * p.parts + G - 1) / G)), dim3(256), 0,
-                     s, m, rows, V, t, ignore, g, p.parts, p.len, dz);
+  hipLaunchKernelGGL((k_score_bwd<T, N, U, W>), grid_of((rows * p.parts + G - 1) / G, 256), dim3(256), 0, s, m, rows, V, t,
+                     ignore, g, p.parts, p.len, dz);
 }
 template <typename T>
 void score_bwd_any(const Rows& m, int64_t rows, int V, const Ids& t, int64_t ignore, const ScoreGrad& g, void* dlogits,

@@ -116,6 +116,9 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
+// the block's number in a grid of grid_of
+__device__ __forceinline__ int64_t block_number() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // f over the 64 lanes, in every lane, on the vector unit alone: lane pairs, quads, eights and
 // rows of 16 by DPP, then rows 0 / 1 and 2 / 3, then the halves.  (Through the LDS crossbar
 // a distillation step of 111,848 rows of 600 values, seven of these each, took 238 us.)
@@ -468,6 +471,13 @@ inline Split map_split(int64_t rows, int64_t V) {
   int64_t len = (V + p - 1) / p;
   len = (len + 511) / 512 * 512;
   return {static_cast<int>((V + len - 1) / len), static_cast<int>(len)};
+}
+
+// HIP takes fewer than 2^32 threads along a grid's x: blocks beyond that go over its y, and the last
+// of them may be past the end.
+inline dim3 grid_of(int64_t blocks, int threads) {
+  const int64_t most = ((int64_t(1) << 32) - 1) / threads, y = (blocks + most - 1) / most;
+  return dim3(static_cast<unsigned>((blocks + y - 1) / y), static_cast<unsigned>(y));
 }
 
 inline bool ids_ok(int bits) { return bits == 8 || bits == 32 || bits == 64; }

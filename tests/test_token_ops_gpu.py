@@ -796,6 +796,62 @@ def test_outputs_of_more_than_2_31_values():
     _grad_near(dz[tail], want, bound, torch.bfloat16, "scores")
 
 
+def _repeats(got, want):
+    """got [n, *want.shape]: every got[i] is want, bit for bit (in slices: got may be large)."""
+    step = max(1, (1 << 30) // max(1, want.numel()))
+    return all(torch.equal(got[a:a + step], want.expand_as(got[a:a + step])) for a in range(0, len(got), step))
+
+
+@pytest.mark.parametrize("V", [33, 300])
+def test_more_rows_than_a_grid_has_threads(V):
+    """More than 2^26 rows of one wave each, 2^32 threads: a batch of rows repeated (expanded
+    logits, no copy) has the bits of that batch alone, in all of its repetitions."""
+    M = _M()
+    n, rows = 16400, 4099
+    z, y = _logits(rows, V, torch.bfloat16, V).to(DEV), _targets(rows, V, V).to(DEV)
+    ids, t = torch.randint(0, V, (rows, 1), device=DEV).int(), torch.randn(rows, 1, device=DEV).bfloat16()
+    zz, yy, ii, tt = z.expand(n, -1, -1), y.int().expand(n, -1), ids.expand(n, -1, -1), t.expand(n, -1, -1)
+    one, many = M.token_logprobs(z, y.int(), top_k=2), M.token_logprobs(zz, yy, top_k=2)
+    assert all(_repeats(a, b) for a, b in zip(many, one))
+    del one, many
+    opts = dict(alpha=0.5, temperature=2.0, reduction="none")
+    assert _repeats(M.distill_loss(zz, ii, tt, yy, **opts), M.distill_loss(z, ids, t, y.int(), **opts))
+    for a, b in zip(M.distill_loss_and_grad(zz, ii, tt, yy, **opts), M.distill_loss_and_grad(z, ids, t, y.int(), **opts)):
+        assert _repeats(a, b)
+    del a, b
+    grads = []
+    for x in (z, zz):
+        leaf = x.detach().requires_grad_()
+        lead = x.shape[:-1]
+        lp = M.token_logprobs(leaf, (y.int().expand(lead))).logprob
+        g = torch.linspace(-1, 1, rows, device=DEV).expand(lead)
+        first = torch.autograd.grad(lp, leaf, g)[0]
+        del lp
+        if V == 33:
+            loss = M.distill_loss(leaf, ids.expand(*lead, -1), t.expand(*lead, -1), y.int().expand(lead), **opts)
+            grads.append((first, torch.autograd.grad(loss, leaf, g)[0]))
+            del loss
+        else:
+            grads.append((first,))
+        del first
+    assert all(_repeats(b, a) for a, b in zip(*grads))
+
+
+def test_more_table_rows_than_a_grid_has_threads():
+    """A lookup of more than 2^24 rows that take a block each."""
+    M = _M()
+    N, V, D = (1 << 24) + 5, 9, 4128
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2 * N * D + (4 << 30):
+        pytest.skip("an output of 139 GB")
+    w = torch.randn(V, D, device=DEV).bfloat16()
+    tok = torch.randint(0, V, (N,), device=DEV)
+    out = M.scaled_embedding(tok.int(), w, 2.0)
+    at = torch.cat([torch.arange(2000, device=DEV), torch.randint(0, N, (50000,), device=DEV),
+                    torch.arange(N - 2000, N, device=DEV)])
+    assert torch.equal(out[at], (w * 2)[tok[at]])
+
+
 def test_second_gradient_is_refused():
     M = _M()
     z = torch.randn(3, 9, device=DEV, requires_grad=True)
