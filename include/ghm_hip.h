@@ -630,7 +630,8 @@ int ghm_zsc_logits(const float* i_emb, int64_t n_rows, const float* t_emb, int D
  *
  * A row whose target is ignore_index is padding: its logits are not used, its
  * results and gradient are 0 (top_id -1).  A target outside 0 .. V - 1 makes its own
- * row NaN.  A logit of -inf has probability 0; a row whose maximum is not finite has no
+ * row's log probability or loss NaN, and what is differentiated through that (entropy and
+ * alternatives do not depend on a target and stay).  A logit of -inf has probability 0; a row whose maximum is not finite has no
  * distribution and is NaN, as log_softmax has it. */
 #define GHM_TOP_MAX 64        /* alternatives ghm_token_logprobs ranks per row */
 #define GHM_DISTILL_MAX 1024  /* teacher entries per row of ghm_distill */

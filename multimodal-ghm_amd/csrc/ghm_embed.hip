@@ -69,7 +69,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(Ids tok, const T* __restrict
 // N * D values in vectors of VE from its first 16-byte boundary on, 256 * U of them per
 // block, so that lines are written whole and past the caches, whatever D is.  A vector that crosses
 // from a row into the next is put together from the one's last VE values and the other's
-// first.  131,071 x 1001 f32 in 102 us (5.1 TB/s; 129 row by row), 131,071 x 2047 bf16
+// first.  131,071 x 1001 f32 in 102 us (5.1 TB/s; 129 row by row; 144 us right after a gradient
+// of the same size, whose lines are still to be written back), 131,071 x 2047 bf16
 // in 114 (151); what fits the 256 MB cache is sooner there by rows: 10,000 x 1001 f32 in 11 us
 // (21), 100,000 x 1001 bf16 in 41 (51).
 constexpr int64_t RUN_BYTES = int64_t(1) << 28;
@@ -486,9 +487,10 @@ __global__ __launch_bounds__(256) void k_embed_sums(const uint32_t* __restrict__
       store_cols<T, VE, STREAM>(dw + static_cast<int64_t>(cur) * D, col, D, acc);
     }
   };
-  // Rows are read one step ahead of their sums and kept packed, keys and positions two steps
-  // (16 bytes each: chunks are multiples of U, and the arrays are padded).  Entries past
-  // the end take row 0 and are not used; short rows (D < VE) go without the pipeline.
+  // Rows are read one step ahead of their sums and kept packed; their keys and positions are read
+  // in the same step, so that each step's row loads wait for its position loads (16 bytes each:
+  // chunks are multiples of U, and the arrays are padded).  Entries past the end take row 0 and
+  // are not used.
   static_assert(U == 8, "two 16-byte reads per step");
   u32x4 kn[2], pn[2], row[U];
   uint32_t k[U];

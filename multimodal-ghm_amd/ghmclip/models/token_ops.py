@@ -7,7 +7,7 @@ have no counterpart in the reference.  Logits, tables and gradients are float32,
 bfloat16 or float16 on a HIP device; sums, statistics and losses are float32.  Work
 is issued on the current stream of the tensors' device; nothing synchronises, so
 token ids are not checked on the host: an id outside the vocabulary gives NaN in
-its own row (and adds nothing to an embedding gradient).  Gradients are of first order and
+what depends on it in its own row (and adds nothing to an embedding gradient).  Gradients are of first order and
 reverse mode; a second one and forward-mode tangents raise.
 """
 from collections import namedtuple
@@ -180,8 +180,9 @@ def token_logprobs(logits, targets=None, top_k=0, ignore_index=-100):
     logprob, entropy and top_logprob are differentiable in the logits.
 
     A row whose target is ``ignore_index`` is padding: not read, 0 (top_id -1), gradient
-    0.  A logit of -inf has probability 0; a row without a finite maximum, or with a
-    target outside 0 .. V - 1, is NaN.  top_k <= min(64, V)."""
+    0.  A logit of -inf has probability 0; a row without a finite maximum is NaN.  A target
+    outside 0 .. V - 1 makes its row's logprob NaN, and a gradient through it; entropy and
+    alternatives do not depend on it.  top_k <= min(64, V)."""
     _check_logits(logits)
     if not isinstance(top_k, int) or not 0 <= top_k <= min(GHM_TOP_MAX, logits.shape[-1]):
         raise ValueError(f"top_k: 0 .. min({GHM_TOP_MAX}, V = {logits.shape[-1]}), got {top_k!r}")
