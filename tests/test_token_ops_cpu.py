@@ -94,7 +94,7 @@ LONG = "not 140001 and not 300001 and not 200003 and not 600000 and not 270001 a
 
 @pytest.mark.parametrize("order,fill,select,least", [
     (0, 255, f"(test_score or test_distill) and dtype1 and {ELSEWHERE} and {LONG} and not far_apart", 80),
-    (1, 90, f"test_embedding and dtype0 and {ELSEWHERE} and {LONG}", 60),
+    (1, 90, f"test_embedding and (dtype0 or every_row) and {ELSEWHERE} and {LONG}", 60),
     (2, 255, f"(masks_and_special or special_values or without) and dtype0 and {ELSEWHERE} and {LONG} and not 70001", 15),
 ], ids=["rows", "tables", "any order"])
 def test_on_the_cpu(lib, order, fill, select, least):
