@@ -83,12 +83,12 @@ __device__ __forceinline__ void top_finish(const T* z, int lo, int hi, TopLds<N,
 template <typename T, int N, int W, typename F>
 __device__ __forceinline__ void top_search(const T* z, int lo, int hi, TopLds<N, W>* lds, int k, int w, int lane,
                                            F emit) {
-  uint64_t last = ~uint64_t(0);
+  uint64_t last = 0;  // a NaN of id 0 has the largest key there is: the first search has no bound
   for (int j = 0; j < k; ++j) {
     uint64_t best = 0;
     for (int v = lo + w * 64 + lane; v < hi; v += W * 64) {
       const uint64_t key = top_key(to_f(z[v]), v);
-      best = key < last && key > best ? key : best;
+      best = (j == 0 || key < last) && key > best ? key : best;
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {

@@ -194,6 +194,21 @@ def test_score_masks_and_special_values(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [10, 33, 200, 300, 3000, 9000, 70001])
+def test_score_first_value_nan(V, dtype):
+    """NaN ranks first at every id, the first one too."""
+    M = _M()
+    z = _logits(6, V, dtype, V)
+    z[:, 0] = math.nan
+    z[1, V // 2] = z[2, V - 1] = math.nan
+    z[3, 1] = math.inf
+    z[4, 1:] = -math.inf
+    z[5] = math.nan
+    for k in (1, 3, min(V, 64)):
+        _check_score(z, None, k, M.token_logprobs(z.to(DEV), top_k=k), f"k {k}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [50, 700, 20000])
 def test_score_ties(V, dtype):
     """Few distinct values: the alternatives are the lowest ids of the largest values."""
