@@ -268,7 +268,7 @@ __device__ __forceinline__ void distill_entries(const T* z, T* d, int lo, int hi
     const float x = to_f(z[id]);
     float v = g.two ? g.both(x) : g.one(x), q = 0.f;
     for (int j = 0; j < tc.k; ++j) q += lds.id[j] == id ? lds.q[j] : 0.f;
-    v -= g.A * q;
+    if (g.A != 0.f) v -= g.A * q;  // without the teacher's part its logits are not used, NaN or not
     if (id == y) v -= g.B;
     from_f(d[id], v);
   };
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(64) void k_distill_short(Rows rows, int64_t n_rows,
   for (int v = 0; v < M; ++v) {
     if (v >= V) break;
     const float d = x[v] - a.m;
-    float g = A * (__builtin_amdgcn_exp2f(__builtin_fmaf(d, mix.c2, -l2 * LOG2E)) - q[v]);
+    float g = A == 0.f ? 0.f : A * (__builtin_amdgcn_exp2f(__builtin_fmaf(d, mix.c2, -l2 * LOG2E)) - q[v]);
     if (mix.hard) g += B * (__builtin_amdgcn_exp2f(__builtin_fmaf(d, LOG2E, -l1 * LOG2E)) - (v == y ? 1.f : 0.f));
     from_f(dz[r * V + v], g);
   }

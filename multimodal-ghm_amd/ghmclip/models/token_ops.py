@@ -278,7 +278,7 @@ def distill_loss(logits, top_ids, top_logits, targets=None, *, temperature=1.0, 
     [..., V]; top_ids [..., k] (int32 / int64) and top_logits [..., k]: the teacher's
     alternatives, k <= 1024 (log probabilities, as token_logprobs returns them, serve as
     well); a negative id or a logit of -inf marks an absent entry, repeated ids add up.
-    targets [...]: hard labels, needed for alpha < 1.
+    targets [...]: hard labels, needed for alpha < 1; alpha = 0 leaves the teacher's logits out.
 
     reduction "mean": over the counted rows (0 if there is none) -- those whose target is
     not ``ignore_index``, or without targets those with an entry --; "sum"; "none": one

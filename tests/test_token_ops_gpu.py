@@ -518,6 +518,31 @@ def test_distill_rows_without_a_distribution(V, dtype):
         assert (dz[~bad] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [10, 33, 300, 3000, 40000, 140001])
+def test_distill_without_the_teacher(V, dtype):
+    """alpha = 0 is the hard labels' loss alone, gradient and all, whatever the teacher's logits hold and
+    though the student may have ruled its values out."""
+    M = _M()
+    z, y = _logits(5, V, dtype, V), torch.tensor([0, 1, 2, -100, 3])
+    ids, t = _teacher(5, V, 4, V, ragged=False)
+    t[0, 1], t[1, 2], t[4] = math.nan, math.inf, math.nan
+    z[2, ids[2, 0]] = -math.inf if ids[2, 0] != 2 else z[2, ids[2, 0]]
+    clean = t.nan_to_num(0, 0)
+    for tau in (1.0, 2.0):
+        r = O.distill(z.double(), ids[:, :1], torch.full((5, 1), -math.inf).double(), y, tau, 0.0)
+        on = [z.to(DEV), ids.to(DEV), t.to(DEV), y.to(DEV)]
+        opts = dict(temperature=tau, alpha=0.0, reduction="none")
+        loss, dz = M.distill_loss_and_grad(*on, **opts)
+        _near(loss, r["row_loss"], r["brow_loss"], "loss")
+        _grad_near(dz, r["dz"], r["bdz"] + 4 * O.U * r["dz"].abs(), dtype, "step")
+        leaf = on[0].requires_grad_()
+        got, = torch.autograd.grad(M.distill_loss(leaf, *on[1:], **opts).sum(), leaf)
+        _grad_near(got, r["dz"], r["bdz"] + 4 * O.U * r["dz"].abs(), dtype, "autograd")
+        again = M.distill_loss_and_grad(on[0].detach(), on[1], clean.to(DEV), on[3], **opts)
+        assert torch.equal(again[0], loss) and torch.equal(again[1], dz)
+
+
 def test_distill_nothing_counts():
     M = _M()
     z = _logits(5, 77, torch.float32, 0).to(DEV).requires_grad_()
