@@ -17,7 +17,7 @@ import pytest
 from conftest import ROOT
 
 HERE = os.path.join(ROOT, "tests", "cpu_kernels")
-OUT = os.path.join(ROOT, "build", "cpu_kernels")
+OUT = os.path.join(ROOT, "build", "cpu_kernels" + os.environ.get("PYTEST_XDIST_WORKER", ""))
 CLANG = "/opt/rocm/llvm/bin/clang++"
 ASAN = sorted(glob.glob("/opt/rocm/llvm/lib/clang/*/lib/*/libclang_rt.asan-x86_64.so"))
 FLAGS = ["-std=c++17", "-O1", "-gline-tables-only", "-fPIC", "-Wno-everything", "-Xarch_host", "-fsanitize=address", "-shared-libasan"]
@@ -70,7 +70,8 @@ def _build():
 
 
 def _run(lib, select, order, fill, **more):
-    env = dict(os.environ, **more, CPU_KERNELS=lib, PYTHONPATH=HERE, LANE_ORDER=str(order), LD_PRELOAD=ASAN[-1],
+    env = {k: v for k, v in os.environ.items() if not k.startswith("PYTEST_")}
+    env = dict(env, **more, CPU_KERNELS=lib, PYTHONPATH=HERE, LANE_ORDER=str(order), LD_PRELOAD=ASAN[-1],
                ASAN_OPTIONS="detect_leaks=0:detect_stack_use_after_return=0:allocator_may_return_null=1:"
                             f"max_malloc_fill_size=2147483647:malloc_fill_byte={fill}")
     r = subprocess.run([sys.executable, "-m", "pytest", "-p", "cpu_device", "-p", "no:cacheprovider", "-q", "-x", "-n", "4",
