@@ -658,6 +658,7 @@ int ghm_token_logprobs_bwd(const void* logits, int dtype, int64_t n_inner, int64
  * with a negative id or a logit of -inf are absent; an id >= V makes its row NaN;
  * repeated ids add up), q = softmax(top_logits / temperature) over a row's entries:
  *   row_loss = (1 - alpha) CE(z, target) + alpha temperature^2 KL(q || softmax(z / temperature)).
+ * alpha = 0 leaves the teacher's logits out, whatever they hold.
  * Counted rows: the target is not ignore_index; without targets (alpha = 1), at least
  * one entry is present.  reduction 0: row_loss only; 1: loss[0] = mean over the counted
  * rows (0 if there is none), norm[0] = 1 / their number; 2: loss[0] = sum.  stats

@@ -915,6 +915,71 @@ def test_more_table_rows_than_a_grid_has_threads():
     assert torch.equal(out[at], (w * 2)[tok[at]])
 
 
+def test_one_row_of_2_30_values():
+    """The longest row there may be.  A lane adds 2^30 / (64 parts of 8 waves of 64 lanes) = 2^15 terms, so
+    the sum is off by 2^15 + 100 units relative to itself at most, 2^-8.99."""
+    M = _M()
+    V, rel = 1 << 30, (2 ** 15 + 100) * O.U
+    torch.cuda.empty_cache()
+    z = torch.empty(1, V, dtype=torch.bfloat16, device=DEV).normal_(0, 2, generator=torch.Generator(DEV).manual_seed(1))
+    top = [V // 2 + 3, V - 1, 7]
+    z[0, top] = torch.tensor([20.0, 20.0, 19.0], dtype=torch.bfloat16, device=DEV)
+    got = M.token_logprobs(z, torch.tensor([V - 1], device=DEV), top_k=3)
+    s = t = 0.0
+    for a in range(0, V, 1 << 26):
+        d = z[0, a:a + (1 << 26)].double() - 20
+        s += float(d.exp().sum())
+        t += float((d.exp() * -d).sum())
+    assert got.top_id.tolist() == [top]
+    assert abs(got.logprob.item() + math.log(s)) <= rel + 8 * O.U
+    assert abs(got.entropy.item() - math.log(s) - t / s) <= rel + 2 * rel * t / s + 64 * O.U
+    leaf = z.requires_grad_()
+    dz, = torch.autograd.grad(M.token_logprobs(leaf, torch.tensor([V - 1], device=DEV)).logprob.sum(), leaf)
+    at = torch.tensor([0, 7, 12345, V // 2 + 3, V - 2, V - 1], device=DEV)
+    p = (z.detach()[0, at].double() - 20).exp() / s
+    want = torch.where(at == V - 1, 1.0, 0.0) - p
+    assert ((dz[0, at].double() - want).abs() <= 2 * rel * p + O.round_bound(want, torch.bfloat16) * 2).all()
+    del dz, leaf
+    ids, tl = torch.tensor([[V - 1, 0, V // 2]], device=DEV), torch.tensor([[2.0, 1.0, 0.0]], device=DEV)
+    loss, dz = M.distill_loss_and_grad(z.detach(), ids, tl)
+    q = torch.softmax(tl.double(), -1)
+    zi = z.detach()[0, ids[0]].double()
+    kl = (q * (q.log() - (zi - 20 - math.log(s)))).sum().item()
+    assert abs(loss.item() - kl) <= rel + 64 * O.U * 40
+    assert M.distill_loss(z.detach(), ids, tl).item() == pytest.approx(kl, abs=rel + 64 * O.U * 40)
+    want = (zi - 20).exp() / s - q[0]
+    assert ((dz[0, ids[0]].double() - want).abs() <= 2 * rel * (zi - 20).exp() / s + O.round_bound(want, torch.bfloat16) * 2).all()
+
+
+def test_2_31_rows():
+    """As many rows and tokens as there may be."""
+    M = _M()
+    R = (1 << 31) - 1
+    torch.cuda.empty_cache()
+    z, y = torch.zeros(R, 1, dtype=torch.bfloat16, device=DEV), torch.zeros(R, dtype=torch.uint8, device=DEV)
+    y[-1] = 1
+    got = M.token_logprobs(z, y)
+    assert got.logprob[-1].isnan() and (got.logprob[:-1] == 0).all() and (got.entropy == 0).all()
+    del got, y
+    torch.cuda.empty_cache()
+    ids = torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(R, 1)
+    loss, dz = M.distill_loss_and_grad(z, ids, torch.zeros(1, 1, dtype=torch.bfloat16, device=DEV).expand(R, 1))
+    assert loss == 0 and (dz == 0).all()
+    del loss, dz, z
+    torch.cuda.empty_cache()
+    tok = torch.randint(0, 40, (R,), device=DEV, dtype=torch.uint8)
+    w = torch.randn(40, 1, device=DEV).bfloat16().requires_grad_()
+    out = M.scaled_embedding(tok, w, 2.0)
+    for a in range(0, R, 1 << 28):
+        assert torch.equal(out[a:a + (1 << 28)].detach(), (w.detach() * 2)[tok[a:a + (1 << 28)].long()])
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    n = sum(torch.bincount(tok[a:a + (1 << 28)], minlength=40) for a in range(0, R, 1 << 28))
+    # a chunk's 256 ones are exact, and each of four waves joins 2^31 / 40 / 256 / 4 of them
+    rel = (2 ** 31 / 40 / 1024 + 4) * O.U
+    assert ((dw[:, 0].double() - 2 * n).abs() <= 2 * n * rel + O.round_bound(2 * n.double(), torch.bfloat16)).all()
+    torch.cuda.empty_cache()
+
+
 def test_second_gradient_is_refused():
     M = _M()
     z = torch.randn(3, 9, device=DEV, requires_grad=True)
