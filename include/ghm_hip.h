@@ -564,7 +564,8 @@ int ghm_gemm_reduce(const float* slab, int nsplit, int64_t M, int64_t N, float* 
 int ghm_gemm_reduce_bias(const float* slab, int nsplit, int64_t M, int64_t N, float* D0, float* D1, float* D2,
                          int64_t chunk, const float* bslab, float* bdst, void* stream);
 /* out[n] = sum_m X[m][n] (deterministic two-stage), X [M][N] fp32, N % 4 == 0 and
- * N/4 dividing 256 or >= 256; part scratch of ghm_colsum_part_elems(M, N) floats.
+ * N/4 dividing 256 or >= 256; part scratch of ghm_colsum_part_elems(M', N) floats
+ * for some M' >= M.
  * The bias gradients of the Linear layers and the position-embedding gradient
  * (autograd's sum over batch rows, model.py:291-293, :330-347). */
 int64_t ghm_colsum_part_elems(int64_t M, int64_t N);
@@ -574,7 +575,7 @@ int ghm_colsum(const float* X, int64_t M, int64_t N, float* out, float* part, vo
  * (dense [M][C]; the readout weight and bias gradients from dlogits) or
  * [tok[m] == c] when W is NULL (token ids [M]; the t_embedding / i_embedding
  * gradients, autograd's embedding backward of model.py:238-241 and :444); xrow(m) = (m / rps) * seq_rows + off + m % rps.  Deterministic two
- * stages; part scratch of ghm_wcolsum_part_elems(M, N, C) floats. */
+ * stages; part scratch of ghm_wcolsum_part_elems(M', N, C) floats for some M' >= M. */
 int64_t ghm_wcolsum_part_elems(int64_t M, int64_t N, int C);
 int ghm_wcolsum(const float* W, const uint8_t* tok, int C, const float* X, int64_t rps, int64_t seq_rows, int64_t off,
                 int64_t M, int64_t N, float* out, float* wsum, float* part, void* stream);

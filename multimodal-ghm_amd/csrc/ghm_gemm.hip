@@ -1227,9 +1227,11 @@ extern "C" int ghm_gemm_reduce(const float* slab, int nsplit, int64_t M, int64_t
 }
 
 extern "C" int64_t ghm_colsum_part_elems(int64_t M, int64_t N) {
-  int64_t cb, nc, R;
-  colsum_plan(M, N, cb, nc, R);
-  return nc * N;
+  // enough for fewer rows too: rounding the rows per chunk up leaves fewer chunks for some M than for
+  // a smaller one, so the bound is the most that colsum_plan starts from
+  const int64_t cb = N / 4 < 256 ? 1 : (N / 4 + 255) / 256, cap = (M + 7) / 8;
+  const int64_t want = 256 / cb > 1 ? 256 / cb : 1, nc = want < cap ? want : cap;
+  return (nc < 1 ? 1 : nc) * N;
 }
 
 extern "C" int ghm_colsum(const float* X, int64_t M, int64_t N, float* out, float* part, void* stream) {
@@ -1263,9 +1265,10 @@ void wcolsum_plan(int64_t M, int64_t& nchunk, int64_t& R) {
 }  // namespace
 
 extern "C" int64_t ghm_wcolsum_part_elems(int64_t M, int64_t N, int C) {
-  int64_t nc, R;
-  wcolsum_plan(M, nc, R);
-  return nc * wcolsum_ldp(N, C);
+  // enough for fewer rows too: 10,368 rows go in 494 chunks, but 10,240 of them (a sequence's rows
+  // without its prefix) in 512
+  const int64_t cap = (M + 7) / 8, nc = cap < 512 ? cap : 512;
+  return (nc < 1 ? 1 : nc) * wcolsum_ldp(N, C);
 }
 
 extern "C" int ghm_wcolsum(const float* W, const uint8_t* tok, int C, const float* X, int64_t rps, int64_t seq_rows,
